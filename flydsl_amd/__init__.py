@@ -11,6 +11,9 @@ Public API (same names and signatures as the reference):
   * kernels/mla_fwd_decode.py: :func:`flydsl_mla_fwd_decode` (MLA fp8 decode),
     with :func:`get_mla_metadata_info_v1`, :func:`get_mla_metadata_v1` and
     :func:`mla_reduce_v1` in place of the aiter calls its test makes.
+and, without a counterpart in the reference,
+  * :func:`pa_decode_shared_prefix`: the decode of a batch whose sequences
+    share prefixes, each read once.
 Device work runs in the hand-written gfx950 HIP kernels of ``libpa_fp8.so``
 (C ABI: ``include/pa_fp8.h``).
 """
@@ -31,6 +34,11 @@ from .mla_decode import (  # noqa: F401
 )
 from .qk_norm_rope import compile_flydsl_qk_norm_rope_quant, flydsl_qk_norm_rope_quant  # noqa: F401
 from .rope_cache import build_fused_rope_cache_module  # noqa: F401
+from .shared_prefix import (  # noqa: F401
+    PreparedSharedPrefix,
+    pa_decode_shared_prefix,
+    prepare_pa_decode_shared_prefix,
+)
 
 __all__ = [
     "pa_decode_ps_launch",
@@ -46,4 +54,7 @@ __all__ = [
     "get_mla_metadata_info_v1",
     "get_mla_metadata_v1",
     "mla_reduce_v1",
+    "pa_decode_shared_prefix",
+    "prepare_pa_decode_shared_prefix",
+    "PreparedSharedPrefix",
 ]

@@ -67,6 +67,9 @@ EXPORTED_SYMBOLS = (
     "pa_fp8_mla_plan_sizes",
     "pa_fp8_mla_plan",
     "pa_fp8_fnuz_to_fn",
+    "pa_fp8_decode_shared_prefix",
+    "pa_fp8_shared_prefix_workspace_bytes",
+    "pa_fp8_plan_shared_prefix",
     "pa_fp8_debug_violations",
     "pa_fp8_checked_build",
 )
@@ -361,6 +364,23 @@ class MlaReduceArgs(ctypes.Structure):
     ]
 
 
+class SharedPrefixArgs(ctypes.Structure):
+    """Mirror of ``pa_fp8_shared_prefix_args`` (field order matters)."""
+
+    _fields_ = (
+        [("abi_version", _i32)]
+        + [(n, _vp) for n in ("output", "query", "key_cache", "value_cache", "block_tables", "context_lengths",
+                              "prefix_indptr", "prefix_lengths", "key_scale", "value_scale")]
+        + [(n, _i64) for n in ("stride_q_tok", "stride_q_head", "stride_k_block", "stride_k_head", "stride_v_block",
+                               "stride_v_head", "stride_bt_seq", "stride_ks_block", "stride_ks_head",
+                               "stride_out_tok", "stride_out_head")]
+        + [(n, _i32) for n in ("num_seqs", "num_groups", "num_kv_heads", "query_length", "query_group_size",
+                               "head_size", "block_size", "num_blocks", "max_blocks_per_seq", "per_token_kv",
+                               "trans_v", "query_dtype", "output_dtype", "num_workers")]
+        + [("softmax_scale", ctypes.c_float)]
+    )
+
+
 class LibraryNotBuilt(RuntimeError):
     pass
 
@@ -433,6 +453,12 @@ def load(path: Optional[str] = None) -> ctypes.CDLL:
     lib.pa_fp8_mla_plan.restype = ctypes.c_int
     lib.pa_fp8_fnuz_to_fn.argtypes = [_vp, _vp, _i64, _i64, _i64, _vp, _vp]
     lib.pa_fp8_fnuz_to_fn.restype = ctypes.c_int
+    lib.pa_fp8_decode_shared_prefix.argtypes = [ctypes.POINTER(SharedPrefixArgs), _vp, _i64, _vp]
+    lib.pa_fp8_decode_shared_prefix.restype = ctypes.c_int
+    lib.pa_fp8_shared_prefix_workspace_bytes.argtypes = [ctypes.c_int] * 7
+    lib.pa_fp8_shared_prefix_workspace_bytes.restype = _i64
+    lib.pa_fp8_plan_shared_prefix.argtypes = [_vp] * 3 + [ctypes.c_int] * 9 + [_vp]
+    lib.pa_fp8_plan_shared_prefix.restype = ctypes.c_int
     lib.pa_fp8_debug_violations.argtypes = [ctypes.POINTER(ctypes.c_uint)]
     lib.pa_fp8_debug_violations.restype = ctypes.c_int
     lib.pa_fp8_checked_build.argtypes = []
@@ -606,3 +632,33 @@ def mla_plan(qo_indptr, kv_indptr, num_workers: int):
     if n < 0:
         check(n, "pa_fp8_mla_plan")
     return n, ng.value, npart.value, out
+
+
+@functools.lru_cache(maxsize=256)
+def shared_prefix_workspace_bytes(num_seqs: int, num_groups: int, num_kv_heads: int, query_length: int,
+                                  query_group_size: int, head_size: int, num_workers: int) -> int:
+    n = int(load().pa_fp8_shared_prefix_workspace_bytes(num_seqs, num_groups, num_kv_heads, query_length,
+                                                        query_group_size, head_size, num_workers))
+    if n < 0:
+        check(n, "pa_fp8_shared_prefix_workspace_bytes")
+    return n
+
+
+def plan_shared_prefix(context_lengths, prefix_indptr, prefix_lengths, num_kv_heads: int, query_length: int,
+                       query_group_size: int, head_size: int, capacity: int, num_workers: int):
+    """Pieces of a shared-prefix decode (numpy int32 [n, 8])."""
+    import numpy as np
+
+    arr = lambda x: np.ascontiguousarray(np.asarray(x, dtype=np.int32))
+    ctx, ptr, ln = arr(context_lengths), arr(prefix_indptr), arr(prefix_lengths)
+    p = lambda a: a.ctypes.data_as(ctypes.c_void_p)
+    out = np.zeros((1, 8), np.int32)
+    for _ in range(2):
+        n = int(load().pa_fp8_plan_shared_prefix(p(ctx), p(ptr), p(ln), len(ctx), len(ln), num_kv_heads, query_length,
+                                                 query_group_size, head_size, capacity, num_workers, len(out), p(out)))
+        if n < 0:
+            check(n, "pa_fp8_plan_shared_prefix")
+        if n <= len(out):
+            break
+        out = np.zeros((n, 8), np.int32)
+    return out[:n]

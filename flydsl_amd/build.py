@@ -11,12 +11,13 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
-SOURCES = [os.path.join(CSRC, n) for n in ("pa_fp8.hip", "rope_cache.hip", "qk_norm_rope.hip", "mla_fp8.hip")]
+SOURCES = [os.path.join(CSRC, n) for n in ("pa_fp8.hip", "rope_cache.hip", "qk_norm_rope.hip", "mla_fp8.hip",
+                                                  "shared_prefix.hip")]
 # MFMA results in VGPRs: the online-softmax rescale and the slot merges of
 # the paged-attention kernels are VALU work on them (no AGPR round trips),
 # and the MLA kernel keeps its logits there while its value accumulators are
 # pinned to AGPRs by inline assembly.
-VGPR_FORM = {"pa_fp8.hip", "rope_cache.hip", "qk_norm_rope.hip", "mla_fp8.hip"}
+VGPR_FORM = {"pa_fp8.hip", "rope_cache.hip", "qk_norm_rope.hip", "mla_fp8.hip", "shared_prefix.hip"}
 # Kernels that must not use scratch: the MLA decode's inline-assembly DMA,
 # waits and hazard cover were written for its register allocation without
 # spills (a build whose extra code made it spill 36 VGPRs returned wrong

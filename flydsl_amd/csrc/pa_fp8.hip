@@ -4985,6 +4985,7 @@ int pa_fp8_debug_violations(unsigned int* bits) {
   if (rc == 0) rc = pa_violations_mla(bits);
   if (rc == 0) rc = pa_violations_rope_cache(bits);
   if (rc == 0) rc = pa_violations_qk_norm_rope(bits);
+  if (rc == 0) rc = pa_violations_shared_prefix(bits);
   return rc;
 }
 
@@ -5357,7 +5358,7 @@ const char* pa_fp8_error_string(int code) {
     case PA_ERR_SHAPE: return "invalid dimension";
     case PA_ERR_ALIGN: return "pointer or stride not 16-byte aligned";
     case PA_ERR_ABI: return "abi_version mismatch";
-    case PA_ERR_SCRATCH: return "the call needs more workspace than the library's static scratch (64 MiB)";
+    case PA_ERR_SCRATCH: return "the call needs more workspace than it was given (or than the library's static scratch, 64 MiB)";
     default: return hipGetErrorString((hipError_t)code);
   }
 }

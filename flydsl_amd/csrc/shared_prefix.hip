@@ -1,0 +1,936 @@
+// Decode attention of a batch whose sequences share prefixes, for MI355X
+// (gfx950): each group's prefix is read once for all of the group's query
+// rows, every sequence's own tokens once for its columns, and the parts are
+// merged by their maxima and sums:
+//   part i of a row:  m_i = max x_j,  l_i = sum 2^(x_j - m_i),
+//                     o_i = sum 2^(x_j - m_i) v_j,   x = q.k scale log2(e)
+//   out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i,   M = max m_i
+//
+// Work decomposition: see sp_plan.h.  One launch of persistent workgroups
+// (eight waves) walks equal shares of the line of prefix and suffix items and
+// leaves float32 pieces; a second launch merges a row's pieces.
+//
+// Arithmetic.  A wave holds NR tiles of 16 query rows and walks 64-token
+// tiles.  Keys and values are fp8 e4m3fn, exact in bf16 and f16, so they are
+// converted and both products run on v_mfma_f32_16x16x32_{bf16,f16}:
+//   S^T = K Q^T   A: 16 tokens x 32 dims, B: Q^T
+//   O^T += V^T P^T  A: 16 dims x 32 tokens, B: P^T
+// Lane (c, g) = (l % 16, l / 16) loads 16-byte pieces straight from the
+// cache's layout: of keys, 16 dims of one token (the k order of S is a
+// permutation of the head dimension that Q shares); of values, the 16 tokens
+// of block g for one dim.  Row m of key tile T is token 16 (m / 4) + 4 T +
+// m % 4, so that the logits lane (c, g) gets from the four tiles are those of
+// row c and the 16 tokens of block g -- the very tokens its value operand
+// holds, and the probabilities need no move between lanes.
+// The probabilities are rounded to the operands' type, by at most 2^-8 (bf16)
+// or 2^-11 (f16) of themselves, as an attention in that type rounds them;
+// sums, maxima and outputs stay in 32 bits.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <vector>
+
+#include "pa_check.h"
+#include "pa_fp8.h"
+#include "sp_plan.h"
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kThreads = 64 * SP_WAVES;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNegInf = -__builtin_inff();
+// A row's reference exponent moves when a logit exceeds it by more than
+// this (base 2): the probabilities stay below 2^8, and most tiles leave the
+// accumulators as they are.
+constexpr float kRescaleMargin = 8.f;
+
+// Everything a launch needs (device side of pa_fp8_shared_prefix_args).
+struct SpArgs {
+  pa_fp8_shared_prefix_args a;
+  SpShape p, s;           // prefix and suffix items
+  int eq, col_tiles;      // query columns per kv head, suffix items per (sequence, kv head)
+  int s_rows;             // rows a suffix piece stores
+  int capacity;           // tokens a table row can hold
+  int lbs;                // log2(page size)
+  // workspace
+  int4* seq_info;         // [B]: first prefix item of the group (-1: none), row of the sequence's first column,
+                          // row tiles of the group, whether the sequence has a suffix
+  int2* items;            // [prefix items, then suffix items]: first slot, pieces
+  int max_prefix_items;
+  float* p_ml;            // [slot][2][rows]
+  float* p_o;             // [slot][rows][D]
+  float* s_ml;
+  float* s_o;
+};
+
+__device__ __forceinline__ float groups_max(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float groups_sum(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Eight fp8 values (two dwords) as an MFMA operand.
+template <bool F16>
+__device__ __forceinline__ i32x4 widen8(int lo, int hi) {
+  union {
+    i32x4 v;
+    bf16x2 b[4];
+    f16x2 h[4];
+  } u;
+  if constexpr (F16) {
+    u.h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
+    u.h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
+    u.h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false);
+    u.h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
+  } else {
+    u.b[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
+    u.b[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
+    u.b[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false);
+    u.b[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+  }
+  return u.v;
+}
+template <bool F16>
+__device__ __forceinline__ int round2(float x, float y) {
+  int r;
+  if constexpr (F16) {
+    f16x2 h = {(_Float16)x, (_Float16)y};
+    __builtin_memcpy(&r, &h, 4);
+  } else {
+    bf16x2 h = {(__bf16)x, (__bf16)y};
+    __builtin_memcpy(&r, &h, 4);
+  }
+  return r;
+}
+template <bool F16>
+__device__ __forceinline__ f32x4 mfma(const i32x4& x, const i32x4& y, const f32x4& c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+}
+
+// Byte mask of a dword whose bytes are tokens t .. t + 3: those in [lo, hi).
+__device__ __forceinline__ uint32_t keep4(int t, int lo, int hi) {
+  const int l = pa_min(pa_max(lo - t, 0), 4), u = pa_min(pa_max(hi - t, l), 4);
+  const uint32_t below_u = u >= 4 ? ~0u : (1u << (8 * u)) - 1;
+  const uint32_t below_l = l >= 4 ? ~0u : (1u << (8 * l)) - 1;
+  return below_u & ~below_l;
+}
+
+// ---------------------------------------------------------------------------
+// The plan of a launch, in LDS
+// ---------------------------------------------------------------------------
+
+struct Plan {
+  int64_t* seq_at;    // [B + 1] cost of the sequences' items before b, one kv head
+  int64_t* group_at;  // [G + 1] likewise of the groups' prefix items
+  int* first;         // [G + 1] first sequence of a group (never falls)
+  int* len;           // [G] prefix length
+  int* row_tiles;     // [G + 1] prefix items of the groups before g, one kv head
+  int64_t* scratch;   // [SP_WAVES]
+};
+
+__host__ __device__ inline int plan_bytes(int B, int G) {
+  return (8 * (B + 1) + 8 * (G + 1) + 8 * SP_WAVES + 4 * (G + 1) + 4 * (G + 1) + 4 * (G + 1) + 15) & ~15;
+}
+__device__ __forceinline__ Plan plan_of(char* lds, int B, int G) {
+  Plan p;
+  p.seq_at = (int64_t*)lds;
+  p.group_at = p.seq_at + B + 1;
+  p.scratch = p.group_at + G + 1;
+  p.first = (int*)(p.scratch + SP_WAVES);
+  p.len = p.first + G + 1;
+  p.row_tiles = p.len + G + 1;
+  return p;
+}
+
+// a[0 .. n] := the sums (MAX: maxima, inclusive) of what stands before each
+// entry; every thread of the workgroup calls it, between barriers of its own.
+template <bool MAX, typename T>
+__device__ void block_scan(T* a, int n, int64_t* scratch) {
+  const int per = (n + kThreads - 1) / kThreads;
+  const int i0 = threadIdx.x * per, i1 = pa_min(i0 + per, n);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  auto op = [](int64_t x, int64_t y) { return MAX ? (x > y ? x : y) : x + y; };
+  __syncthreads();
+  int64_t mine = 0;
+  for (int i = i0; i < i1; ++i) mine = op(mine, (int64_t)a[i]);
+  int64_t upto = mine;
+  for (int d = 1; d < 64; d *= 2) {
+    const int64_t o = __shfl_up((long long)upto, d, 64);
+    if (lane >= d) upto = op(upto, o);
+  }
+  if (lane == 63) scratch[wave] = upto;
+  int64_t before = __shfl_up((long long)upto, 1, 64);
+  if (lane == 0) before = 0;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) before = op(before, scratch[w]);
+  for (int i = i0; i < i1; ++i) {
+    const int64_t v = (int64_t)a[i];
+    if (MAX) {
+      before = op(before, v);
+      a[i] = (T)before;
+    } else {
+      a[i] = (T)before;
+      before += v;
+    }
+  }
+  if (!MAX && i0 < n && i1 == n) a[n] = (T)before;
+  if (!MAX && n == 0 && threadIdx.x == 0) a[0] = 0;
+  __syncthreads();
+}
+
+// Last entry of a[0 .. n] (never falls) that is <= x, for a[0] <= x.
+template <typename T>
+__device__ __forceinline__ int last_le(const T* a, int n, int64_t x) {
+  int lo = 0, hi = n + 1;
+  while (hi - lo > 1) {
+    const int m = (lo + hi) >> 1;
+    if ((int64_t)a[m] <= x)
+      lo = m;
+    else
+      hi = m;
+  }
+  return lo;
+}
+
+// The group of sequence b, or -1.
+__device__ __forceinline__ int group_of(const Plan& p, int G, int b) {
+  if (G <= 0 || b < p.first[0] || b >= p.first[G]) return -1;
+  return last_le(p.first, G, b);
+}
+
+__device__ __forceinline__ int context_of(const SpArgs& s, int b) {
+  const int n = s.a.context_lengths[b];
+  return n < 0 ? 0 : (n < s.capacity ? n : s.capacity);
+}
+
+__device__ void make_plan(const Plan& p, const SpArgs& s) {
+  const int B = s.a.num_seqs, G = s.a.num_groups;
+  if (G > 0) {
+    for (int g = threadIdx.x; g <= G; g += kThreads) p.first[g] = pa_min(pa_max(s.a.prefix_indptr[g], 0), B);
+    block_scan<true>(p.first, G + 1, p.scratch);
+    for (int g = threadIdx.x; g < G; g += kThreads) {
+      const int rows = (p.first[g + 1] - p.first[g]) * s.eq;
+      const int len = rows > 0 ? pa_min(pa_max(s.a.prefix_lengths[g], 0), s.capacity) : 0;
+      const int tiles = len > 0 ? pa_cdiv(rows, s.p.rows) : 0;
+      p.len[g] = len;
+      p.row_tiles[g] = tiles;
+      p.group_at[g] = (int64_t)tiles * sp_item_cost(sp_steps(0, len, s.p.wt), s.p.cost);
+    }
+    block_scan<false>(p.row_tiles, G, p.scratch);
+    block_scan<false>(p.group_at, G, p.scratch);
+  } else if (threadIdx.x == 0) {
+    p.group_at[0] = 0;
+  }
+  for (int b = threadIdx.x; b < B; b += kThreads) {
+    const int g = group_of(p, G, b);
+    const int len = g >= 0 ? p.len[g] : 0;
+    p.seq_at[b] = (int64_t)s.col_tiles * sp_item_cost(sp_steps(len, context_of(s, b), s.s.wt), s.s.cost);
+  }
+  block_scan<false>(p.seq_at, B, p.scratch);
+}
+
+// ---------------------------------------------------------------------------
+// One piece
+// ---------------------------------------------------------------------------
+
+struct Piece {
+  bool prefix;
+  int b0;            // sequence whose table row gives the pages, and of the item's row 0
+  int row0, nrows;   // first row of the item among the group's rows (the sequence's columns), and their count
+  int h;             // kv head
+  int begin, end;    // tokens of the item
+  int tile, tile_end;  // tiles of the piece
+  int wt, waves_r, rows_out;
+  float* ml;         // the slot
+  float* o;
+};
+
+// LDS of the pieces' ends: maxima and sums by wave, then 32 output dims.
+constexpr int kOutStride = 36;  // floats a row of 32 dims takes (16-byte steps that spread over the banks)
+__host__ __device__ constexpr int end_bytes(int nr) {
+  return SP_WAVES * 16 * nr * 4 * 2 + SP_WAVES * 16 * nr * kOutStride * 4;
+}
+
+template <int D, bool F16, bool PT, int NR>
+__device__ __forceinline__ void run_piece(const SpArgs& s, const Piece& pc, char* lds) {
+  // the value product of f16 queries with per-token scales runs in bf16: a
+  // scale of any size times a probability stays in range
+  constexpr bool PF16 = F16 && !PT;
+  const pa_fp8_shared_prefix_args& a = s.a;
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wave / pc.wt, wi = wave - wr * pc.wt;
+  const int eq = s.eq, ql = a.query_length, gqa = a.query_group_size;
+  const int bs = 1 << s.lbs;
+
+  // ---- query rows ----
+  const float c0 = a.softmax_scale * kLog2e * (PT ? 1.0f : a.key_scale[0]);
+  const float fac = c0 == 0.0f ? 1.0f : fabsf(c0);
+  const int flip = c0 < 0.0f ? (int)0x80008000u : 0, keep = c0 == 0.0f ? 0 : -1;
+  i32x4 q[NR][D / 32];
+  int limit[NR];  // keys the row sees: below it
+  int least = 0x7fffffff;
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    const int r = pc.row0 + (wr * NR + n) * 16 + c;
+    const bool live = r < pc.nrows;
+    const int bb = live ? r / eq : 0, e = live ? r - bb * eq : 0;
+    const int b = pc.b0 + bb, qi = e / gqa;
+    limit[n] = 0x7fffffff;
+    if (live) {
+      const int ctx = a.context_lengths[b];
+      limit[n] = pa_min(pa_max(ctx - ql + qi + 1, 0), pc.end);
+    }
+    least = pa_min(least, limit[n]);
+    const uint16_t* row = (const uint16_t*)a.query + (int64_t)(b * (int64_t)ql + qi) * a.stride_q_tok +
+                          (int64_t)(pc.h * gqa + (e - qi * gqa)) * a.stride_q_head;
+#pragma unroll
+    for (int u = 0; u < D / 64; ++u)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        i32x4 w = {0, 0, 0, 0};
+        if (live) w = *(const i32x4*)(row + (4 * u + g) * 16 + 8 * k);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (w[i] ^ flip) & keep;
+        q[n][2 * u + k] = w;
+      }
+  }
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) least = pa_min(least, __shfl_xor(least, d, 64));
+  least = __builtin_amdgcn_readfirstlane(least);
+
+  // ---- addresses ----
+  const int32_t* table = a.block_tables + (int64_t)pc.b0 * a.stride_bt_seq;
+  const int last_page = pa_min((pc.end - 1) >> s.lbs, a.max_blocks_per_seq - 1);
+  const uint8_t* kbase = (const uint8_t*)a.key_cache + (int64_t)pc.h * a.stride_k_head;
+  const uint8_t* vbase = (const uint8_t*)a.value_cache + (int64_t)pc.h * a.stride_v_head;
+  const int v_dim = a.trans_v ? 16 : bs, v_blk = a.trans_v ? D * 16 : 16;
+  auto page_of = [&](int token) -> int {
+    int p = table[pa_min(token >> s.lbs, last_page)];
+    pa_note(p < 0 || p >= a.num_blocks, PA_VIOLATION_PAGE);
+    p = p < 0 ? 0 : p;
+    return p < a.num_blocks ? p : a.num_blocks - 1;
+  };
+  const int kblk = c >> 2;  // the lane's key tokens are of block kblk, its value tokens of block g
+  i32x4 kr[4][D / 64], vr[D / 16];
+  f32x4 ks[4], vs[4];
+  auto load_keys = [&](int tile, int page) {
+    const int in = ((tile * SP_TILE + 16 * kblk) & (bs - 1)) + (c & 3);
+    const uint8_t* p = kbase + (int64_t)page * a.stride_k_block + in * 16 + g * (bs * 16);
+#pragma unroll
+    for (int T = 0; T < 4; ++T)
+#pragma unroll
+      for (int u = 0; u < D / 64; ++u) kr[T][u] = *(const i32x4*)(p + 64 * T + (int64_t)(4 * u) * (bs * 16));
+  };
+  auto load_values = [&](int tile, int page) {
+    const int in = ((tile * SP_TILE + 16 * g) & (bs - 1)) >> 4;
+    const uint8_t* p = vbase + (int64_t)page * a.stride_v_block + in * v_blk + c * v_dim;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) vr[dt] = *(const i32x4*)(p + (int64_t)(16 * dt) * v_dim);
+  };
+  auto load_scales = [&](const float* base, int tile, int page, f32x4 (&x)[4]) {
+    const float* p = base + (int64_t)page * a.stride_ks_block + (int64_t)pc.h * a.stride_ks_head +
+                     ((tile * SP_TILE + 16 * g) & (bs - 1));
+#pragma unroll
+    for (int T = 0; T < 4; ++T) x[T] = *(const f32x4*)(p + 4 * T);
+  };
+
+  f32x4 o[NR][D / 16];
+  float m[NR], l[NR];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    m[n] = kNegInf;
+    l[n] = 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) o[n][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  int tile = pc.tile + wi;
+  int kp = 0, vp = 0;
+  if (tile < pc.tile_end) {
+    kp = page_of(tile * SP_TILE + 16 * kblk);
+    vp = page_of(tile * SP_TILE + 16 * g);
+    load_keys(tile, kp);
+    load_values(tile, vp);
+    if constexpr (PT) {
+      load_scales(a.key_scale, tile, vp, ks);
+      load_scales(a.value_scale, tile, vp, vs);
+    }
+    const int next = pa_min(tile + pc.wt, pc.tile_end - 1);
+    kp = page_of(next * SP_TILE + 16 * kblk);
+    vp = page_of(next * SP_TILE + 16 * g);
+  }
+  for (; tile < pc.tile_end; tile += pc.wt) {
+    const int next = tile + pc.wt;
+    const bool more = next < pc.tile_end;
+    // ---- logits of tokens 16 g + 4 T + i ----
+    f32x4 x[NR][4];
+#pragma unroll
+    for (int T = 0; T < 4; ++T) {
+#pragma unroll
+      for (int n = 0; n < NR; ++n) x[n][T] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < D / 64; ++u) {
+        const i32x4 k0 = widen8<F16>(kr[T][u][0], kr[T][u][1]), k1 = widen8<F16>(kr[T][u][2], kr[T][u][3]);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          x[n][T] = mfma<F16>(k0, q[n][2 * u], x[n][T]);
+          x[n][T] = mfma<F16>(k1, q[n][2 * u + 1], x[n][T]);
+        }
+      }
+    }
+    if (more) load_keys(next, kp);
+    if constexpr (PT) {
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int T = 0; T < 4; ++T) x[n][T] *= ks[T];
+      if (more) load_scales(a.key_scale, next, vp, ks);
+    }
+    // ---- masks: the part's first and last tiles ----
+    const int t0 = tile * SP_TILE;
+    if (t0 < pc.begin || t0 + SP_TILE > pa_min(least, pc.end)) {
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int T = 0; T < 4; ++T)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int t = t0 + 16 * g + 4 * T + i;
+            if (t < pc.begin || t >= limit[n]) x[n][T][i] = kNegInf;
+          }
+      // bytes behind the part's tokens may be anything, NaN among it
+#pragma unroll
+      for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vr[dt][i] &= (int)keep4(t0 + 16 * g + 4 * i, pc.begin, pc.end);
+      if constexpr (PT) {
+#pragma unroll
+        for (int T = 0; T < 4; ++T)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int t = t0 + 16 * g + 4 * T + i;
+            if (t < pc.begin || t >= pc.end) vs[T][i] = 0.0f;
+          }
+      }
+    }
+    // ---- softmax ----
+    i32x4 p[NR][2];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      float top = kNegInf;
+#pragma unroll
+      for (int T = 0; T < 4; ++T)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, x[n][T][i]);
+      top = groups_max(top) * fac;
+      if (__ballot(top > m[n] + kRescaleMargin)) {
+        const float mn = fmaxf(m[n], top);
+        const float f = mn == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m[n] - mn);
+        l[n] *= f;
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) o[n][dt] *= f;
+        m[n] = mn;
+      }
+      const float bias = m[n] == kNegInf ? 0.0f : -m[n];
+      float w[16];
+#pragma unroll
+      for (int T = 0; T < 4; ++T)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][T][i], fac, bias));
+          l[n] += e;
+          w[4 * T + i] = PT ? e * vs[T][i] : e;
+        }
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[n][j][i] = round2<PF16>(w[8 * j + 2 * i], w[8 * j + 2 * i + 1]);
+    }
+    // ---- values ----
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) {
+      const i32x4 v0 = widen8<PF16>(vr[dt][0], vr[dt][1]), v1 = widen8<PF16>(vr[dt][2], vr[dt][3]);
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        o[n][dt] = mfma<PF16>(v0, p[n][0], o[n][dt]);
+        o[n][dt] = mfma<PF16>(v1, p[n][1], o[n][dt]);
+      }
+    }
+    if (more) {
+      load_values(next, vp);
+      if constexpr (PT) load_scales(a.value_scale, next, vp, vs);
+      const int after = pa_min(next + pc.wt, pc.tile_end - 1);
+      kp = page_of(after * SP_TILE + 16 * kblk);
+      vp = page_of(after * SP_TILE + 16 * g);
+    }
+  }
+
+  // ---- the waves of the same rows, merged; the piece written ----
+  float* lm = (float*)lds;                       // [wave][16 NR]
+  float* ll = lm + SP_WAVES * 16 * NR;
+  float* lo = ll + SP_WAVES * 16 * NR;           // [wave][16 NR][kOutStride]
+  __syncthreads();                               // the piece before has been read
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    l[n] = groups_sum(l[n]);
+    if (g == 0) {
+      lm[(wave * NR + n) * 16 + c] = m[n];
+      ll[(wave * NR + n) * 16 + c] = l[n];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    float top = kNegInf, sum = 0.0f;
+    for (int w = wr * pc.wt; w < (wr + 1) * pc.wt; ++w) top = fmaxf(top, lm[(w * NR + n) * 16 + c]);
+    for (int w = wr * pc.wt; w < (wr + 1) * pc.wt; ++w) {
+      const float mw = lm[(w * NR + n) * 16 + c];
+      sum += mw == kNegInf ? ll[(w * NR + n) * 16 + c] * 0.0f : ll[(w * NR + n) * 16 + c] * __builtin_amdgcn_exp2f(mw - top);
+    }
+    const float f = m[n] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m[n] - top);
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) o[n][dt] *= f;
+    const int r = (wr * NR + n) * 16 + c;
+    if (wi == 0 && g == 0 && pc.row0 + r < pc.nrows) {
+      pc.ml[r] = top;
+      pc.ml[pc.rows_out + r] = sum;
+    }
+  }
+  const int rows_wg = pc.waves_r * 16 * NR;
+#pragma unroll
+  for (int d0 = 0; d0 < D / 32; ++d0) {
+    if (d0) __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        *(f32x4*)(lo + ((wave * NR + n) * 16 + c) * kOutStride + 16 * k + 4 * g) = o[n][2 * d0 + k];
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows_wg * 8; i += kThreads) {
+      const int r = i >> 3, d = (i & 7) * 4;
+      if (pc.row0 + r >= pc.nrows) break;  // (rows only grow with i)
+      const int w0 = r / (16 * NR) * pc.wt, rr = r % (16 * NR);
+      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+      for (int w = w0; w < w0 + pc.wt; ++w) sum += *(const f32x4*)(lo + (w * 16 * NR + rr) * kOutStride + d);
+      *(f32x4*)(pc.o + (int64_t)r * D + 32 * d0 + d) = sum;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The kernels
+// ---------------------------------------------------------------------------
+
+template <int D, bool F16, bool PT>
+__global__ __launch_bounds__(kThreads, 2) void pa_shared_prefix_kernel(const SpArgs s) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const pa_fp8_shared_prefix_args& a = s.a;
+  const int B = a.num_seqs, G = a.num_groups, H = a.num_kv_heads;
+  const Plan pl = plan_of(lds, B, G);
+  char* const work = lds + plan_bytes(B, G);
+  make_plan(pl, s);
+
+  // what the merge needs of each sequence
+  const int worker = blockIdx.x;
+  for (int b = worker + (int)gridDim.x * (int)threadIdx.x; b < B; b += (int)gridDim.x * kThreads) {
+    const int gr = group_of(pl, G, b);
+    const bool has = gr >= 0 && pl.len[gr] > 0;
+    int4 v;
+    v.x = has ? H * pl.row_tiles[gr] : -1;
+    v.y = has ? (b - pl.first[gr]) * s.eq : 0;
+    v.z = has ? pl.row_tiles[gr + 1] - pl.row_tiles[gr] : 0;
+    v.w = pl.seq_at[b + 1] > pl.seq_at[b];
+    s.seq_info[b] = v;
+  }
+
+  const int64_t prefix_line = (int64_t)H * pl.group_at[G], line = prefix_line + (int64_t)H * pl.seq_at[B];
+  if (line == 0) return;
+  const int W = sp_workers(line, gridDim.x);
+  if (worker >= W) return;
+  int64_t at = sp_begin(worker, line, W);
+  const int64_t lo = at, hi = sp_begin(worker + 1, line, W);
+  const int slots_p = s.max_prefix_items;
+
+  // prefix items
+  while (at < hi && at < prefix_line) {
+    const int gr = last_le(pl.group_at, G, at / H);
+    const int tiles = pl.row_tiles[gr + 1] - pl.row_tiles[gr];
+    const int steps = sp_steps(0, pl.len[gr], s.p.wt);
+    const int cost = sp_item_cost(steps, s.p.cost);
+    const int64_t g_at = (int64_t)H * pl.group_at[gr];
+    const int idx = (int)((at - g_at) / cost);  // kv head outer, row tile inner
+    const int64_t i_at = g_at + (int64_t)idx * cost;
+    const int s0 = sp_step_from(lo, i_at, steps, s.p.cost), s1 = sp_step_from(hi, i_at, steps, s.p.cost);
+    at = i_at + cost;
+    if (s1 <= s0) continue;
+    const int item = H * pl.row_tiles[gr] + idx;
+    Piece pc;
+    pc.prefix = true;
+    pc.b0 = __builtin_amdgcn_readfirstlane(pl.first[gr]);
+    pc.h = __builtin_amdgcn_readfirstlane(idx / tiles);
+    pc.row0 = __builtin_amdgcn_readfirstlane((idx % tiles) * s.p.rows);
+    pc.nrows = __builtin_amdgcn_readfirstlane((pl.first[gr + 1] - pl.first[gr]) * s.eq);
+    pc.begin = 0;
+    pc.end = __builtin_amdgcn_readfirstlane(pl.len[gr]);
+    pc.tile = __builtin_amdgcn_readfirstlane(s0 * s.p.wt);
+    pc.tile_end = __builtin_amdgcn_readfirstlane(pa_min(s1 * s.p.wt, pa_cdiv(pc.end, SP_TILE)));
+    pc.wt = s.p.wt;
+    pc.waves_r = s.p.waves_r;
+    pc.rows_out = s.p.rows;
+    const int slot = __builtin_amdgcn_readfirstlane(item + worker);
+    pc.ml = s.p_ml + (int64_t)slot * 2 * s.p.rows;
+    pc.o = s.p_o + (int64_t)slot * s.p.rows * D;
+    if (s0 == 0 && threadIdx.x == 0) {
+      const int last = sp_worker_of(i_at + SP_OVERHEAD + (int64_t)(steps - 1) * s.p.cost, line, W);
+      s.items[item] = int2{item + worker, last - worker + 1};
+    }
+    if constexpr (D <= 128) {
+      if (s.p.nr == 2)
+        run_piece<D, F16, PT, 2>(s, pc, work);
+      else
+        run_piece<D, F16, PT, 1>(s, pc, work);
+    } else {
+      run_piece<D, F16, PT, 1>(s, pc, work);
+    }
+  }
+  // suffix items
+  while (at < hi) {
+    const int64_t rel = at - prefix_line;
+    const int b = last_le(pl.seq_at, B, rel / H);
+    const int gr = group_of(pl, G, b);
+    const int begin = gr >= 0 ? pl.len[gr] : 0, end = context_of(s, b);
+    const int steps = sp_steps(begin, end, s.s.wt);
+    const int cost = sp_item_cost(steps, s.s.cost);
+    const int64_t b_at = (int64_t)H * pl.seq_at[b];
+    const int idx = (int)((rel - b_at) / cost);  // kv head outer, column tile inner
+    const int64_t i_at = prefix_line + b_at + (int64_t)idx * cost;
+    const int s0 = sp_step_from(lo, i_at, steps, s.s.cost), s1 = sp_step_from(hi, i_at, steps, s.s.cost);
+    at = i_at + cost;
+    if (s1 <= s0) continue;
+    const int item = b * H * s.col_tiles + idx;
+    Piece pc;
+    pc.prefix = false;
+    pc.b0 = __builtin_amdgcn_readfirstlane(b);
+    pc.h = __builtin_amdgcn_readfirstlane(idx / s.col_tiles);
+    pc.row0 = __builtin_amdgcn_readfirstlane((idx % s.col_tiles) * s.s.rows);
+    pc.nrows = s.eq;
+    pc.begin = __builtin_amdgcn_readfirstlane(begin);
+    pc.end = __builtin_amdgcn_readfirstlane(end);
+    const int base = pc.begin / SP_TILE;
+    pc.tile = base + __builtin_amdgcn_readfirstlane(s0 * s.s.wt);
+    pc.tile_end = pa_min(base + __builtin_amdgcn_readfirstlane(s1 * s.s.wt), pa_cdiv(pc.end, SP_TILE));
+    pc.wt = s.s.wt;
+    pc.waves_r = s.s.waves_r;
+    pc.rows_out = s.s_rows;
+    const int slot = __builtin_amdgcn_readfirstlane(item + worker);
+    pc.ml = s.s_ml + (int64_t)slot * 2 * s.s_rows;
+    pc.o = s.s_o + (int64_t)slot * s.s_rows * D;
+    if (s0 == 0 && threadIdx.x == 0) {
+      const int last = sp_worker_of(i_at + SP_OVERHEAD + (int64_t)(steps - 1) * s.s.cost, line, W);
+      s.items[slots_p + item] = int2{item + worker, last - worker + 1};
+    }
+    if constexpr (D <= 128) {
+      if (s.s.nr == 2)
+        run_piece<D, F16, PT, 2>(s, pc, work);
+      else
+        run_piece<D, F16, PT, 1>(s, pc, work);
+    } else {
+      run_piece<D, F16, PT, 1>(s, pc, work);
+    }
+  }
+}
+
+constexpr int kMergeThreads = 256;
+
+// out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over a row's pieces.
+// Workgroup (sequence and kv head, block of columns): D / 4 threads hold a
+// row's four dims each; where the block has fewer columns than the workgroup
+// has such teams, several teams share a row's pieces and meet in LDS.
+template <int D, bool PT>
+__global__ __launch_bounds__(kMergeThreads) void pa_shared_prefix_merge_kernel(const SpArgs s, int block_cols) {
+  constexpr int kTeam = D / 4, kTeams = kMergeThreads / kTeam;
+  __shared__ float lm[kTeams], ll[kTeams];
+  __shared__ __attribute__((aligned(16))) f32x4 lo[kMergeThreads];
+  const pa_fp8_shared_prefix_args& a = s.a;
+  const int H = a.num_kv_heads, b = blockIdx.x / H, h = blockIdx.x - b * H;
+  const int team = threadIdx.x / kTeam, d = (threadIdx.x - team * kTeam) * 4;
+  const int shares = kTeams / block_cols;  // teams a column
+  const int col = team / shares, share = team - col * shares;
+  const int e = blockIdx.y * block_cols + col;
+  const bool live = team < shares * block_cols && e < s.eq;
+
+  const int4 info = s.seq_info[b];
+  float m = kNegInf, l = 0.0f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  auto take = [&](const float* ml, const float* po, int rows, int slot, int pieces, int r) {
+    for (int i = share; i < pieces; i += shares) {
+      const int64_t at = slot + i;
+      const float mi = ml[at * 2 * rows + r], li = ml[at * 2 * rows + rows + r];
+      const f32x4 oi = *(const f32x4*)(po + (at * rows + r) * D + d);
+      const float mn = fmaxf(m, mi);
+      const float f = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+      const float fi = mi == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mi - mn);
+      l = l * f + li * fi;
+      o = o * f + oi * fi;
+      m = mn;
+    }
+  };
+  if (live) {
+    if (info.x >= 0) {
+      const int row = info.y + e, t = row / s.p.rows;
+      const int2 it = s.items[info.x + h * info.z + t];
+      take(s.p_ml, s.p_o, s.p.rows, it.x, it.y, row - t * s.p.rows);
+    }
+    if (info.w) {
+      const int t = e / s.s.rows;
+      const int2 it = s.items[s.max_prefix_items + (b * H + h) * s.col_tiles + t];
+      take(s.s_ml, s.s_o, s.s_rows, it.x, it.y, e - t * s.s.rows);
+    }
+  }
+  if (shares > 1) {
+    if (d == 0) {
+      lm[team] = m;
+      ll[team] = l;
+    }
+    lo[threadIdx.x] = o;
+    __syncthreads();
+    if (!live || share) return;
+    for (int i = 1; i < shares; ++i) {
+      const float mi = lm[team + i], mn = fmaxf(m, mi);
+      const float f = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+      const float fi = mi == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mi - mn);
+      l = l * f + ll[team + i] * fi;
+      o = o * f + lo[threadIdx.x + i * kTeam] * fi;
+      m = mn;
+    }
+  }
+  if (!live) return;
+  // a row that sees no key is zero
+  const float f = l == 0.0f ? 0.0f : (PT ? 1.0f : a.value_scale[0]) / l;
+  const int qi = e / a.query_group_size;
+  const int64_t off = (int64_t)(b * (int64_t)a.query_length + qi) * a.stride_out_tok +
+                      (int64_t)(h * a.query_group_size + e - qi * a.query_group_size) * a.stride_out_head + d;
+  if (l == 0.0f) o = f32x4{0.f, 0.f, 0.f, 0.f};
+  o *= f;
+  if (a.output_dtype == PA_DTYPE_F32)
+    *(f32x4*)((float*)a.output + off) = o;
+  else if (a.output_dtype == PA_DTYPE_F16)
+    *(int2*)((uint16_t*)a.output + off) = int2{round2<true>(o[0], o[1]), round2<true>(o[2], o[3])};
+  else
+    *(int2*)((uint16_t*)a.output + off) = int2{round2<false>(o[0], o[1]), round2<false>(o[2], o[3])};
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+
+struct Sizes {
+  SpShape p, s;
+  int eq, col_tiles, s_rows;
+  int64_t prefix_items, suffix_items;
+  int64_t seq_info, items, p_ml, p_o, s_ml, s_o, total;  // byte offsets
+};
+
+bool head_ok(int d) { return d == 64 || d == 128 || d == 192 || d == 256; }
+
+// Sizes of a launch; 0 or a PA_ERR_* code.
+int sizes_of(int B, int G, int H, int ql, int gqa, int D, int workers, Sizes* z) {
+  if (!head_ok(D)) return PA_ERR_HEAD_SIZE;
+  if (B < 0 || G < 0 || H <= 0 || ql <= 0 || gqa <= 0 || workers <= 0 || B > SP_MAX_SEQS || G > SP_MAX_GROUPS)
+    return PA_ERR_SHAPE;
+  const int64_t eq = (int64_t)ql * gqa, rows = eq * B;
+  if (eq > (1 << 20) || rows > 0x7fffffff || (int64_t)H * gqa > 0x7fffffff) return PA_ERR_SHAPE;
+  z->eq = (int)eq;
+  z->s = sp_shape((int)eq, D);
+  z->col_tiles = (int)((eq + z->s.rows - 1) / z->s.rows);
+  z->s_rows = z->col_tiles > 1 ? z->s.rows : (int)eq;
+  z->p = sp_shape((int)((rows + pa_max(G, 1) - 1) / pa_max(G, 1)), D);
+  z->prefix_items = G > 0 ? (rows / z->p.rows + pa_min(G, B)) * H : 0;
+  z->suffix_items = (int64_t)B * H * z->col_tiles;
+  if (z->prefix_items + workers > 0x7fffffff / 2 || z->suffix_items + workers > 0x7fffffff / 2) return PA_ERR_SHAPE;
+  int64_t at = 0;
+  auto take = [&](int64_t n) {
+    const int64_t here = at;
+    at = (at + n + 255) & ~(int64_t)255;
+    return here;
+  };
+  const int64_t np = z->prefix_items > 0 ? z->prefix_items + workers : 0, ns = z->suffix_items + workers;
+  z->seq_info = take(16 * (int64_t)B);
+  z->items = take(8 * (z->prefix_items + z->suffix_items));
+  z->p_ml = take(np * 8 * z->p.rows);
+  z->s_ml = take(ns * 8 * z->s_rows);
+  z->p_o = take(np * z->p.rows * D * 4);
+  z->s_o = take(ns * z->s_rows * D * 4);
+  z->total = at;
+  return PA_OK;
+}
+
+template <int D, bool F16, bool PT>
+hipError_t launch(const SpArgs& s, hipStream_t st) {
+  const int lds = plan_bytes(s.a.num_seqs, s.a.num_groups) + end_bytes(pa_max(s.p.nr, s.s.nr));
+  hipLaunchKernelGGL((pa_shared_prefix_kernel<D, F16, PT>), dim3(s.a.num_workers), dim3(kThreads), lds, st, s);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  constexpr int teams = kMergeThreads / (D / 4);
+  int cols = 1;
+  while (cols < teams && cols < s.eq) cols *= 2;
+  if (cols > teams) cols = teams;
+  hipLaunchKernelGGL((pa_shared_prefix_merge_kernel<D, PT>),
+                     dim3((unsigned)(s.a.num_seqs * s.a.num_kv_heads), (unsigned)pa_cdiv(s.eq, cols)),
+                     dim3(kMergeThreads), 0, st, s, cols);
+  return hipGetLastError();
+}
+
+template <int D>
+hipError_t dispatch(const SpArgs& s, hipStream_t st) {
+  const bool f16 = s.a.query_dtype == PA_DTYPE_F16;
+  if (s.a.per_token_kv) return f16 ? launch<D, true, true>(s, st) : launch<D, false, true>(s, st);
+  return f16 ? launch<D, true, false>(s, st) : launch<D, false, false>(s, st);
+}
+
+bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
+}  // namespace
+
+PA_CHECK_DEFINE_TAKE(pa_violations_shared_prefix)
+
+extern "C" int64_t pa_fp8_shared_prefix_workspace_bytes(int num_seqs, int num_groups, int num_kv_heads,
+                                                        int query_length, int query_group_size, int head_size,
+                                                        int num_workers) {
+  Sizes z;
+  const int rc = sizes_of(num_seqs, num_groups, num_kv_heads, query_length, query_group_size, head_size, num_workers, &z);
+  return rc == PA_OK ? z.total : rc;
+}
+
+extern "C" int pa_fp8_plan_shared_prefix(const int32_t* context_lengths, const int32_t* prefix_indptr,
+                                         const int32_t* prefix_lengths, int B, int G, int H, int ql, int gqa, int D,
+                                         int capacity, int workers, int max_pieces, int32_t* pieces) {
+  Sizes z;
+  const int rc = sizes_of(B, G, H, ql, gqa, D, workers, &z);
+  if (rc != PA_OK) return rc;
+  if ((B > 0 && !context_lengths) || (G > 0 && (!prefix_indptr || !prefix_lengths)) || (max_pieces > 0 && !pieces))
+    return PA_ERR_NULL_ARG;
+  std::vector<int> first(G + 1, 0), len(G, 0), tiles(G + 1, 0), seq_len(B, 0);
+  int top = 0;
+  for (int g = 0; g <= G && G > 0; ++g) first[g] = top = pa_max(top, pa_min(pa_max(prefix_indptr[g], 0), B));
+  struct Kind {
+    bool prefix;
+    int of, h0, items, begin, steps, end, base;
+  };
+  std::vector<Kind> line;
+  int64_t total = 0;
+  for (int g = 0; g < G; ++g) {
+    const int rows = (first[g + 1] - first[g]) * z.eq;
+    len[g] = rows > 0 ? pa_min(pa_max(prefix_lengths[g], 0), capacity) : 0;
+    for (int b = first[g]; b < first[g + 1]; ++b) seq_len[b] = len[g];
+    tiles[g + 1] = tiles[g] + (len[g] > 0 ? pa_cdiv(rows, z.p.rows) : 0);
+    const int n = tiles[g + 1] - tiles[g], steps = sp_steps(0, len[g], z.p.wt);
+    if (n > 0) line.push_back({true, g, n, H * n, 0, steps, len[g], H * tiles[g]});
+    total += (int64_t)H * n * sp_item_cost(steps, z.p.cost);
+  }
+  for (int b = 0; b < B; ++b) {
+    const int end = pa_min(pa_max(context_lengths[b], 0), capacity);
+    const int steps = sp_steps(seq_len[b], end, z.s.wt);
+    if (steps > 0) line.push_back({false, b, z.col_tiles, H * z.col_tiles, seq_len[b], steps, end, b * H * z.col_tiles});
+    total += (int64_t)H * z.col_tiles * sp_item_cost(steps, z.s.cost);
+  }
+  if (total == 0) return 0;
+  const int W = sp_workers(total, workers);
+  int n = 0;
+  int64_t at = 0;
+  for (const Kind& k : line) {
+    const SpShape& sh = k.prefix ? z.p : z.s;
+    for (int i = 0; i < k.items; ++i) {
+      const int w0 = sp_worker_of(at + SP_OVERHEAD, total, W);
+      const int w1 = sp_worker_of(at + SP_OVERHEAD + (int64_t)(k.steps - 1) * sh.cost, total, W);
+      for (int w = w0; w <= w1; ++w) {
+        const int s0 = sp_step_from(sp_begin(w, total, W), at, k.steps, sh.cost);
+        const int s1 = sp_step_from(sp_begin(w + 1, total, W), at, k.steps, sh.cost);
+        if (n < max_pieces) {
+          const int t0 = k.begin / SP_TILE;
+          const int32_t rec[8] = {k.prefix, k.base + i, w, k.base + i + w, k.of, i / k.h0, t0 + s0 * sh.wt,
+                                  pa_min(t0 + s1 * sh.wt, pa_cdiv(k.end, SP_TILE))};
+          for (int j = 0; j < 8; ++j) pieces[8 * n + j] = rec[j];
+        }
+        ++n;
+      }
+      at += sp_item_cost(k.steps, sh.cost);
+    }
+  }
+  return n;
+}
+
+extern "C" int pa_fp8_decode_shared_prefix(const pa_fp8_shared_prefix_args* a, void* workspace,
+                                           int64_t workspace_bytes, void* stream) {
+  if (!a) return PA_ERR_NULL_ARG;
+  if (a->abi_version != PA_FP8_ABI_VERSION) return PA_ERR_ABI;
+  Sizes z;
+  const int rc = sizes_of(a->num_seqs, a->num_groups, a->num_kv_heads, a->query_length, a->query_group_size,
+                          a->head_size, a->num_workers, &z);
+  if (rc != PA_OK) return rc;
+  const int bs = a->block_size;
+  if (bs < 16 || bs > 1024 || (bs & (bs - 1))) return PA_ERR_BLOCK_SIZE;
+  if (a->num_blocks < 0 || a->max_blocks_per_seq < 0) return PA_ERR_SHAPE;
+  if (a->query_dtype != PA_DTYPE_BF16 && a->query_dtype != PA_DTYPE_F16) return PA_ERR_DTYPE;
+  if (a->output_dtype != PA_DTYPE_BF16 && a->output_dtype != PA_DTYPE_F16 && a->output_dtype != PA_DTYPE_F32)
+    return PA_ERR_DTYPE;
+  if (a->num_seqs == 0) return PA_OK;
+  if (a->num_blocks == 0 || a->max_blocks_per_seq == 0) return PA_ERR_SHAPE;
+  if (!a->output || !a->query || !a->key_cache || !a->value_cache || !a->block_tables || !a->context_lengths ||
+      !a->key_scale || !a->value_scale || !workspace || (a->num_groups > 0 && (!a->prefix_indptr || !a->prefix_lengths)))
+    return PA_ERR_NULL_ARG;
+  // 16-byte vectors of queries (8 values), cache bytes, scales (4) and outputs (4)
+  if (!al16(a->query) || !al16(a->key_cache) || !al16(a->value_cache) || !al16(a->output) || !al16(workspace) ||
+      a->stride_q_tok % 8 || a->stride_q_head % 8 || a->stride_k_block % 16 || a->stride_k_head % 16 ||
+      a->stride_v_block % 16 || a->stride_v_head % 16 || a->stride_out_tok % 4 || a->stride_out_head % 4)
+    return PA_ERR_ALIGN;
+  if (a->per_token_kv && (!al16(a->key_scale) || !al16(a->value_scale) || a->stride_ks_block % 4 || a->stride_ks_head % 4))
+    return PA_ERR_ALIGN;
+  if (workspace_bytes < z.total) return PA_ERR_SCRATCH;
+  if ((int64_t)a->num_seqs * a->num_kv_heads > 0x7fffffff || pa_cdiv(z.eq, 2) > 65535) return PA_ERR_SHAPE;
+  SpArgs s;
+  s.a = *a;
+  s.p = z.p;
+  s.s = z.s;
+  s.eq = z.eq;
+  s.col_tiles = z.col_tiles;
+  s.s_rows = z.s_rows;
+  const int64_t cap = (int64_t)a->max_blocks_per_seq * bs;
+  s.capacity = cap < (1 << 30) ? (int)cap : 1 << 30;
+  s.lbs = 31 - __builtin_clz((unsigned)bs);
+  char* ws = (char*)workspace;
+  s.seq_info = (int4*)(ws + z.seq_info);
+  s.items = (int2*)(ws + z.items);
+  s.max_prefix_items = (int)z.prefix_items;
+  s.p_ml = (float*)(ws + z.p_ml);
+  s.p_o = (float*)(ws + z.p_o);
+  s.s_ml = (float*)(ws + z.s_ml);
+  s.s_o = (float*)(ws + z.s_o);
+  hipStream_t st = (hipStream_t)stream;
+  hipError_t e;
+  switch (a->head_size) {
+    case 64: e = dispatch<64>(s, st); break;
+    case 128: e = dispatch<128>(s, st); break;
+    case 192: e = dispatch<192>(s, st); break;
+    default: e = dispatch<256>(s, st); break;
+  }
+  return e == hipSuccess ? PA_OK : (int)e;
+}

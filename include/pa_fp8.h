@@ -74,7 +74,8 @@ enum pa_fp8_error {
   PA_ERR_SHAPE = -6,          /* non-positive dimension or partition count */
   PA_ERR_ALIGN = -7,          /* a pointer or stride breaks 16-byte alignment */
   PA_ERR_ABI = -8,            /* struct abi_version mismatch */
-  PA_ERR_SCRATCH = -9,        /* workspace beyond the static scratch of pa_fp8_decode_balanced_static */
+  PA_ERR_SCRATCH = -9,        /* workspace beyond the static scratch of pa_fp8_decode_balanced_static, or
+                               * smaller than the entry point's *_workspace_bytes */
 };
 
 /*
@@ -612,6 +613,80 @@ int pa_fp8_mla_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, int num_
  */
 int pa_fp8_fnuz_to_fn(const void* src, const int32_t* rows, int64_t num_rows, int64_t num_src_rows,
                       int64_t row_bytes, void* dst, void* hip_stream);
+
+/*
+ * Decode attention of a batch whose sequences share prefixes.  No counterpart
+ * in the reference.
+ *
+ * The result is that of a decode over block_tables and context_lengths (query
+ * qi of a sequence of n tokens sees keys 0 .. n - ql + qi).  Group g is the
+ * sequences prefix_indptr[g] .. prefix_indptr[g + 1] - 1, whose first
+ * prefix_lengths[g] tokens are the same: they are read once for the group,
+ * through the table row of its first sequence, the tokens behind them through
+ * each sequence's own row.  Any prefix length is taken (it need not end with a
+ * page); sequences outside the groups share nothing.  Group bounds are clamped
+ * to [0, num_seqs] and to never fall, lengths to what a table row can hold.
+ * Rows that see no key are zero.
+ *
+ * Head sizes 64, 128, 192 and 256; page sizes 16, 32, ..., 1024 (powers of
+ * two); at most 4096 sequences and 1024 groups.  Two launches; the workspace
+ * (pa_fp8_shared_prefix_workspace_bytes) needs no initialisation and is the
+ * call's own until the launches end.  num_workers: persistent workgroups, one
+ * per compute unit.  16-byte alignment: query strides are multiples of 8
+ * elements, cache strides of 16 bytes, output and per-token scale strides of 4
+ * elements.
+ */
+typedef struct pa_fp8_shared_prefix_args {
+  int32_t abi_version; /* = PA_FP8_ABI_VERSION */
+  void* output;
+  const void* query;
+  const void* key_cache;
+  const void* value_cache;
+  const int32_t* block_tables;
+  const int32_t* context_lengths;
+  const int32_t* prefix_indptr;  /* [num_groups + 1] */
+  const int32_t* prefix_lengths; /* [num_groups] */
+  const float* key_scale;
+  const float* value_scale;
+  /* element strides */
+  int64_t stride_q_tok, stride_q_head;
+  int64_t stride_k_block, stride_k_head;
+  int64_t stride_v_block, stride_v_head;
+  int64_t stride_bt_seq;
+  int64_t stride_ks_block, stride_ks_head; /* per-token scales only */
+  int64_t stride_out_tok, stride_out_head;
+  /* sizes */
+  int32_t num_seqs;
+  int32_t num_groups;
+  int32_t num_kv_heads;
+  int32_t query_length;
+  int32_t query_group_size;
+  int32_t head_size;
+  int32_t block_size;
+  int32_t num_blocks;
+  int32_t max_blocks_per_seq;
+  int32_t per_token_kv;
+  int32_t trans_v;
+  int32_t query_dtype;
+  int32_t output_dtype;
+  int32_t num_workers;
+  float softmax_scale;
+} pa_fp8_shared_prefix_args;
+
+int64_t pa_fp8_shared_prefix_workspace_bytes(int num_seqs, int num_groups, int num_kv_heads, int query_length,
+                                             int query_group_size, int head_size, int num_workers);
+int pa_fp8_decode_shared_prefix(const pa_fp8_shared_prefix_args* args, void* workspace, int64_t workspace_bytes,
+                                void* hip_stream);
+/*
+ * The pieces those launches work, on the host: records of eight int32 (1 for a
+ * prefix piece or 0, item, worker, slot, group or sequence, kv head, first
+ * tile, end tile; tiles of 64 tokens) in the order of the line, at most
+ * max_pieces of them.  Returns their number or a PA_ERR_* code.
+ */
+int pa_fp8_plan_shared_prefix(const int32_t* context_lengths, const int32_t* prefix_indptr,
+                              const int32_t* prefix_lengths, int num_seqs, int num_groups, int num_kv_heads,
+                              int query_length, int query_group_size, int head_size, int capacity, int num_workers,
+                              int max_pieces, int32_t* pieces);
 
 /*
  * Checked builds.  libpa_fp8_checked.so is built from the same sources with
