@@ -13,11 +13,21 @@ Public API (same names and signatures as the reference):
     :func:`mla_reduce_v1` in place of the aiter calls its test makes.
 and, without a counterpart in the reference,
   * :func:`pa_decode_shared_prefix`: the decode of a batch whose sequences
-    share prefixes, each read once.
+    share prefixes, each read once;
+  * :func:`copy_cache_pages`, :func:`fork_cache_pages`,
+    :func:`extend_cache_pages`, :func:`free_cache_pages` and
+    :func:`compact_cache_pages`: the pages of the caches it reads.
 Device work runs in the hand-written gfx950 HIP kernels of ``libpa_fp8.so``
 (C ABI: ``include/pa_fp8.h``).
 """
 
+from .cache_pages import (  # noqa: F401
+    compact_cache_pages,
+    copy_cache_pages,
+    extend_cache_pages,
+    fork_cache_pages,
+    free_cache_pages,
+)
 from .pa_decode import (  # noqa: F401
     KV_COMPUTE_BLOCK,
     PreparedDecode,
@@ -57,4 +67,9 @@ __all__ = [
     "pa_decode_shared_prefix",
     "prepare_pa_decode_shared_prefix",
     "PreparedSharedPrefix",
+    "copy_cache_pages",
+    "fork_cache_pages",
+    "extend_cache_pages",
+    "free_cache_pages",
+    "compact_cache_pages",
 ]

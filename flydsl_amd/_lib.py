@@ -70,6 +70,12 @@ EXPORTED_SYMBOLS = (
     "pa_fp8_decode_shared_prefix",
     "pa_fp8_shared_prefix_workspace_bytes",
     "pa_fp8_plan_shared_prefix",
+    "pa_fp8_pages_workspace_bytes",
+    "pa_fp8_copy_pages",
+    "pa_fp8_fork_pages",
+    "pa_fp8_extend_pages",
+    "pa_fp8_free_pages",
+    "pa_fp8_compact_pages",
     "pa_fp8_debug_violations",
     "pa_fp8_checked_build",
 )
@@ -381,6 +387,28 @@ class SharedPrefixArgs(ctypes.Structure):
     )
 
 
+class PageTableArgs(ctypes.Structure):
+    """Mirror of ``pa_fp8_page_table_args`` (field order matters)."""
+
+    _fields_ = (
+        [("abi_version", _i32), ("block_tables", _vp), ("context_lengths", _vp), ("ref_counts", _vp),
+         ("stride_bt_seq", _i64)]
+        + [(n, _i32) for n in ("num_rows", "max_blocks_per_seq", "num_blocks", "block_size")]
+    )
+
+
+class PageCache(ctypes.Structure):
+    """Mirror of ``pa_fp8_page_cache`` (field order matters)."""
+
+    _fields_ = [("data", _vp), ("stride_bytes", _i64), ("page_bytes", _i64)]
+
+
+# Operations of pa_fp8_pages_workspace_bytes.
+PAGES_COPY = 0
+PAGES_EXTEND = 1
+PAGES_COMPACT = 2
+
+
 class LibraryNotBuilt(RuntimeError):
     pass
 
@@ -459,6 +487,19 @@ def load(path: Optional[str] = None) -> ctypes.CDLL:
     lib.pa_fp8_shared_prefix_workspace_bytes.restype = _i64
     lib.pa_fp8_plan_shared_prefix.argtypes = [_vp] * 3 + [ctypes.c_int] * 9 + [_vp]
     lib.pa_fp8_plan_shared_prefix.restype = ctypes.c_int
+    table, caches = ctypes.POINTER(PageTableArgs), ctypes.POINTER(PageCache)
+    lib.pa_fp8_pages_workspace_bytes.argtypes = [ctypes.c_int] * 3
+    lib.pa_fp8_pages_workspace_bytes.restype = _i64
+    lib.pa_fp8_copy_pages.argtypes = [caches, ctypes.c_int, ctypes.c_int, _vp, _vp, ctypes.c_int, _vp, _vp, _i64, _vp]
+    lib.pa_fp8_copy_pages.restype = ctypes.c_int
+    lib.pa_fp8_fork_pages.argtypes = [table, _vp, _vp, ctypes.c_int, _vp, _vp]
+    lib.pa_fp8_fork_pages.restype = ctypes.c_int
+    lib.pa_fp8_extend_pages.argtypes = [table, caches, ctypes.c_int, _vp, _vp, ctypes.c_int, _vp, _vp, _i64, _vp]
+    lib.pa_fp8_extend_pages.restype = ctypes.c_int
+    lib.pa_fp8_free_pages.argtypes = [table, _vp, _vp, ctypes.c_int, _vp, _vp]
+    lib.pa_fp8_free_pages.restype = ctypes.c_int
+    lib.pa_fp8_compact_pages.argtypes = [table, caches, ctypes.c_int, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp]
+    lib.pa_fp8_compact_pages.restype = ctypes.c_int
     lib.pa_fp8_debug_violations.argtypes = [ctypes.POINTER(ctypes.c_uint)]
     lib.pa_fp8_debug_violations.restype = ctypes.c_int
     lib.pa_fp8_checked_build.argtypes = []
@@ -474,7 +515,9 @@ _NATIVE_ENTRIES = (
     "pa_fp8_split_slot_bytes", "pa_fp8_team_slot_bytes", "pa_fp8_decode_balanced", "pa_fp8_merge_balanced",
     "pa_fp8_balanced_workspace_bytes", "pa_fp8_decode_worklist", "pa_fp8_reduce_worklist",
     "pa_fp8_recommended_splits", "pa_fp8_rope_cache", "pa_fp8_qk_norm_rope_quant", "pa_fp8_mla_decode",
-    "pa_fp8_mla_reduce",
+    "pa_fp8_mla_reduce", "pa_fp8_decode_shared_prefix", "pa_fp8_shared_prefix_workspace_bytes",
+    "pa_fp8_pages_workspace_bytes", "pa_fp8_copy_pages", "pa_fp8_fork_pages", "pa_fp8_extend_pages",
+    "pa_fp8_free_pages", "pa_fp8_compact_pages",
 )
 _NATIVE = None
 
@@ -642,6 +685,14 @@ def shared_prefix_workspace_bytes(num_seqs: int, num_groups: int, num_kv_heads: 
     if n < 0:
         check(n, "pa_fp8_shared_prefix_workspace_bytes")
     return n
+
+
+@functools.lru_cache(maxsize=256)
+def pages_workspace_bytes(operation: int, num_blocks: int, n: int) -> int:
+    b = int(load().pa_fp8_pages_workspace_bytes(operation, num_blocks, n))
+    if b < 0:
+        check(b, "pa_fp8_pages_workspace_bytes")
+    return b
 
 
 def plan_shared_prefix(context_lengths, prefix_indptr, prefix_lengths, num_kv_heads: int, query_length: int,

@@ -12,7 +12,7 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 SOURCES = [os.path.join(CSRC, n) for n in ("pa_fp8.hip", "rope_cache.hip", "qk_norm_rope.hip", "mla_fp8.hip",
-                                                  "shared_prefix.hip")]
+                                                  "shared_prefix.hip", "cache_pages.hip")]
 # MFMA results in VGPRs: the online-softmax rescale and the slot merges of
 # the paged-attention kernels are VALU work on them (no AGPR round trips),
 # and the MLA kernel keeps its logits there while its value accumulators are

@@ -19,6 +19,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstring>
+#include <vector>
 
 #include "pa_fp8.h"
 
@@ -41,6 +42,14 @@ struct Entry {
   decltype(&pa_fp8_qk_norm_rope_quant) qknr;
   decltype(&pa_fp8_mla_decode) mla_decode;
   decltype(&pa_fp8_mla_reduce) mla_reduce;
+  decltype(&pa_fp8_decode_shared_prefix) shared_prefix;
+  decltype(&pa_fp8_shared_prefix_workspace_bytes) shared_prefix_bytes;
+  decltype(&pa_fp8_pages_workspace_bytes) pages_bytes;
+  decltype(&pa_fp8_copy_pages) copy_pages;
+  decltype(&pa_fp8_fork_pages) fork_pages;
+  decltype(&pa_fp8_extend_pages) extend_pages;
+  decltype(&pa_fp8_free_pages) free_pages;
+  decltype(&pa_fp8_compact_pages) compact_pages;
 } fn;
 bool ready = false;
 PyObject* check_fn = nullptr;  // _lib.check(rc, name): raises
@@ -777,6 +786,322 @@ PyObject* mla_reduce(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---------------------------------------------------------------------------
+// Shared-prefix decode
+// ---------------------------------------------------------------------------
+
+// The current stream, where the tensors' device is the current one too (a
+// launch on the null stream goes to the current device).
+bool current_here(int dev, hipStream_t* s) {
+  int64_t id;
+  int cur = -1;
+  return hipGetDevice(&cur) == hipSuccess && cur == dev && current(dev, s, &id);
+}
+
+// shared_prefix(output, query, key_cache, value_cache, context_lengths, block_tables, prefix_indptr, prefix_lengths,
+//               softmax_scale, key_scale, value_scale, workers); workers(device index) -> workgroups
+PyObject* shared_prefix(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 12) NOT_HERE;
+  return guarded([&]() -> PyObject* {
+    Reader rd;
+    const at::Tensor* t[8];
+    for (int i = 0; i < 8; ++i) t[i] = rd(a[i]);
+    const at::Tensor *ks = rd(a[9]), *vs = rd(a[10]);
+    if (!rd.ok || !PyFloat_CheckExact(a[8])) NOT_HERE;
+    const at::Tensor &out = *t[0], &q = *t[1], &kc = *t[2], &vc = *t[3], &cl = *t[4], &bt = *t[5], &ip = *t[6], &pl = *t[7];
+    if (q.dim() != 3 || kc.dim() != 5 || cl.dim() != 1 || bt.dim() != 2 || ip.dim() != 1 || pl.dim() != 1) NOT_HERE;
+    const bool bf16 = is(q, at::kBFloat16);
+    if (!bf16 && !is(q, at::kHalf)) NOT_HERE;
+    int od;
+    if (is(out, at::kBFloat16)) od = PA_DTYPE_BF16;
+    else if (is(out, at::kHalf)) od = PA_DTYPE_F16;
+    else if (is(out, at::kFloat)) od = PA_DTYPE_F32;
+    else NOT_HERE;
+    const int64_t B = cl.size(0), G = pl.size(0), rows = q.size(0), Hq = q.size(1), D = q.size(2), NB = kc.size(0),
+                  H = kc.size(1), bs = kc.size(3), M = bt.size(1);
+    if (B <= 0 || B > 4096 || G > 1024 || rows == 0 || rows % B || H <= 0 || Hq <= 0 || Hq % H || NB <= 0 || M <= 0)
+      NOT_HERE;
+    if (D % 64 || D < 64 || D > 256 || bs < 16 || bs > 1024 || (bs & (bs - 1))) NOT_HERE;
+    const int64_t lim = 0x7fffffff;
+    if (rows > lim || NB > lim || M > lim || Hq > lim) NOT_HERE;
+    if (!shape_is(kc, {NB, H, D / 16, bs, 16})) NOT_HERE;
+    const bool trans = vc.dim() == 5;
+    if (trans ? !shape_is(vc, {NB, H, bs / 16, D, 16}) : !shape_is(vc, {NB, H, D, bs})) NOT_HERE;
+    for (const at::Tensor* x : {&kc, &vc})
+      if (!is(*x, at::kFloat8_e4m3fn) && !is(*x, at::kByte)) NOT_HERE;
+    if (kc.stride(4) != 1 || kc.stride(3) != 16 || kc.stride(2) != bs * 16) NOT_HERE;
+    if (trans ? !(vc.stride(4) == 1 && vc.stride(3) == 16 && (bs == 16 || vc.stride(2) == D * 16))
+              : !(vc.stride(3) == 1 && vc.stride(2) == bs))
+      NOT_HERE;
+    if (q.stride(2) != 1 || out.sizes() != q.sizes() || out.stride(2) != 1 || bt.stride(1) != 1 || bt.size(0) < B) NOT_HERE;
+    if (!is(cl, at::kInt) || !is(bt, at::kInt) || !is(ip, at::kInt) || !is(pl, at::kInt) || !cl.is_contiguous() ||
+        !ip.is_contiguous() || !pl.is_contiguous() || ip.size(0) != G + 1)
+      NOT_HERE;
+    if (!is(*ks, at::kFloat) || !is(*vs, at::kFloat)) NOT_HERE;
+    const bool pt = ks->dim() > 1;
+    if (pt) {
+      if (!shape_is(*ks, {NB, H, bs, 1}) || !shape_is(*vs, {NB, H, bs, 1}) || ks->strides() != vs->strides() ||
+          ks->stride(2) != 1)
+        NOT_HERE;
+    } else if (vs->dim() > 1 || ks->numel() != 1 || vs->numel() != 1) {
+      NOT_HERE;
+    }
+    hipStream_t s;
+    if (!current_here(rd.dev, &s)) NOT_HERE;
+    PyObject* w = PyObject_CallFunction(a[11], "i", rd.dev);
+    if (!w) return nullptr;
+    const long workers = PyLong_AsLong(w);
+    Py_DECREF(w);
+    if (PyErr_Occurred()) return nullptr;
+    pa_fp8_shared_prefix_args r;
+    std::memset(&r, 0, sizeof r);
+    r.abi_version = PA_FP8_ABI_VERSION;
+    r.output = out.data_ptr();
+    r.query = q.data_ptr();
+    r.key_cache = kc.data_ptr();
+    r.value_cache = vc.data_ptr();
+    r.block_tables = (const int32_t*)bt.data_ptr();
+    r.context_lengths = (const int32_t*)cl.data_ptr();
+    r.prefix_indptr = (const int32_t*)ip.data_ptr();
+    r.prefix_lengths = G ? (const int32_t*)pl.data_ptr() : nullptr;
+    r.key_scale = (const float*)ks->data_ptr();
+    r.value_scale = (const float*)vs->data_ptr();
+    r.stride_q_tok = q.stride(0);
+    r.stride_q_head = q.stride(1);
+    r.stride_k_block = kc.stride(0);
+    r.stride_k_head = kc.stride(1);
+    r.stride_v_block = vc.stride(0);
+    r.stride_v_head = vc.stride(1);
+    r.stride_bt_seq = bt.stride(0);
+    if (pt) {
+      r.stride_ks_block = ks->stride(0);
+      r.stride_ks_head = ks->stride(1);
+    }
+    r.stride_out_tok = out.stride(0);
+    r.stride_out_head = out.stride(1);
+    r.num_seqs = (int32_t)B;
+    r.num_groups = (int32_t)G;
+    r.num_kv_heads = (int32_t)H;
+    r.query_length = (int32_t)(rows / B);
+    r.query_group_size = (int32_t)(Hq / H);
+    r.head_size = (int32_t)D;
+    r.block_size = (int32_t)bs;
+    r.num_blocks = (int32_t)NB;
+    r.max_blocks_per_seq = (int32_t)M;
+    r.per_token_kv = pt;
+    r.trans_v = trans;
+    r.query_dtype = bf16 ? PA_DTYPE_BF16 : PA_DTYPE_F16;
+    r.output_dtype = od;
+    r.num_workers = (int32_t)workers;
+    r.softmax_scale = (float)PyFloat_AS_DOUBLE(a[8]);
+    const int64_t bytes = fn.shared_prefix_bytes(r.num_seqs, r.num_groups, r.num_kv_heads, r.query_length,
+                                                 r.query_group_size, r.head_size, r.num_workers);
+    if (bytes < 0) NOT_HERE;
+    const at::Tensor ws = device_bytes(bytes, rd.dev);
+    const int rc = launch([&] { return fn.shared_prefix(&r, ws.data_ptr(), bytes, s); });
+    if (rc != 0) return failed(rc, "pa_fp8_decode_shared_prefix");
+    Py_RETURN_TRUE;
+  });
+}
+
+// ---------------------------------------------------------------------------
+// Page operators
+// ---------------------------------------------------------------------------
+
+// A list of `entries` (-1: any, then set) contiguous int32 values, or false.
+bool int_list(const at::Tensor* t, int64_t most, int64_t* entries) {
+  if (!is(*t, at::kInt) || t->dim() != 1 || !t->is_contiguous() || t->size(0) > most || t->size(0) == 0) return false;
+  if (*entries < 0) *entries = t->size(0);
+  return t->size(0) == *entries;
+}
+
+// Caches of a list or tuple; false where Python has to look.
+bool read_caches(PyObject* o, Reader& rd, int64_t* pages, std::vector<pa_fp8_page_cache>* out) {
+  if (!PyList_CheckExact(o) && !PyTuple_CheckExact(o)) return false;
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(o);
+  out->resize((size_t)n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const at::Tensor* t = rd(PySequence_Fast_GET_ITEM(o, i));
+    if (!t || !rd.ok || t->dim() < 2) return false;
+    if (*pages < 0) *pages = t->size(0);
+    if (t->size(0) != *pages || *pages <= 0) return false;
+    int64_t dense = 1;  // elements of a page that lie together
+    for (int64_t d = t->dim() - 1; d > 0; --d) {
+      if (t->size(d) != 1 && t->stride(d) != dense) return false;
+      dense *= t->size(d);
+    }
+    if (dense == 0) return false;
+    pa_fp8_page_cache& c = (*out)[(size_t)i];
+    const int64_t size = (int64_t)t->element_size();
+    c.data = t->data_ptr();
+    c.page_bytes = dense * size;
+    c.stride_bytes = *pages > 1 ? t->stride(0) * size : c.page_bytes;
+    if (c.stride_bytes < c.page_bytes || c.page_bytes > (1 << 30)) return false;
+  }
+  return true;
+}
+
+bool read_table(PyObject* bt, PyObject* cl, PyObject* rc, PyObject* bs, Reader& rd, pa_fp8_page_table_args* a) {
+  const at::Tensor *t = rd(bt), *l = rd(cl), *r = rd(rc);
+  if (!rd.ok || !PyLong_CheckExact(bs)) return false;
+  const int64_t size = PyLong_AsLongLong(bs);
+  if (PyErr_Occurred()) return PyErr_Clear(), false;
+  if (size < 1 || size > (1 << 20) || (size & (size - 1))) return false;
+  if (!is(*t, at::kInt) || !is(*l, at::kInt) || !is(*r, at::kInt) || t->dim() != 2 || l->dim() != 1 || r->dim() != 1 ||
+      !l->is_contiguous() || !r->is_contiguous())
+    return false;
+  const int64_t rows = t->size(0), width = t->size(1), pages = r->size(0), lim = 0x7fffffff;
+  if (rows <= 0 || width <= 0 || pages <= 0 || rows > lim || width > lim || pages > (4 << 20) || l->size(0) != rows)
+    return false;
+  if ((width > 1 && t->stride(1) != 1) || (rows > 1 && t->stride(0) < width)) return false;
+  std::memset(a, 0, sizeof *a);
+  a->abi_version = PA_FP8_ABI_VERSION;
+  a->block_tables = (int32_t*)t->data_ptr();
+  a->context_lengths = (int32_t*)l->data_ptr();
+  a->ref_counts = (int32_t*)r->data_ptr();
+  a->stride_bt_seq = t->stride(0);
+  a->num_rows = (int32_t)rows;
+  a->max_blocks_per_seq = (int32_t)width;
+  a->num_blocks = (int32_t)pages;
+  a->block_size = (int32_t)size;
+  return true;
+}
+
+at::Tensor device_ints(at::IntArrayRef shape, int dev) {
+  return at::empty(shape, at::TensorOptions().dtype(at::kInt).device(at::Device(at::kCUDA, (c10::DeviceIndex)dev)));
+}
+
+// copy_pages(caches, source_pages, target_pages) -> status
+PyObject* copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 3) NOT_HERE;
+  return guarded([&]() -> PyObject* {
+    Reader rd;
+    std::vector<pa_fp8_page_cache> caches;
+    int64_t pages = -1, m = -1;
+    const at::Tensor *src = rd(a[1]), *dst = rd(a[2]);
+    if (!rd.ok || !int_list(src, 65536, &m) || !int_list(dst, 65536, &m)) NOT_HERE;
+    if (!read_caches(a[0], rd, &pages, &caches) || caches.empty() || pages > 0x7fffffff) NOT_HERE;
+    hipStream_t s;
+    if (!current_here(rd.dev, &s)) NOT_HERE;
+    const at::Tensor status = device_ints({m}, rd.dev);
+    const int64_t bytes = m > 64 ? fn.pages_bytes(PA_PAGES_COPY, 0, (int)m) : 0;
+    at::Tensor ws;
+    if (bytes > 0) ws = device_bytes(bytes, rd.dev);
+    const int rc = launch([&] {
+      return fn.copy_pages(caches.data(), (int)caches.size(), (int)pages, (const int32_t*)src->data_ptr(),
+                           (const int32_t*)dst->data_ptr(), (int)m, (int32_t*)status.data_ptr(),
+                           bytes > 0 ? ws.data_ptr() : nullptr, bytes, s);
+    });
+    if (rc != 0) return failed(rc, "pa_fp8_copy_pages");
+    return THPVariable_Wrap(status);
+  });
+}
+
+// fork_pages(block_tables, context_lengths, ref_counts, parents, children, block_size) -> status
+PyObject* fork_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 6) NOT_HERE;
+  return guarded([&]() -> PyObject* {
+    Reader rd;
+    pa_fp8_page_table_args t;
+    int64_t m = -1;
+    if (!read_table(a[0], a[1], a[2], a[5], rd, &t)) NOT_HERE;
+    const at::Tensor *p = rd(a[3]), *c = rd(a[4]);
+    if (!rd.ok || !int_list(p, 65536, &m) || !int_list(c, 65536, &m)) NOT_HERE;
+    hipStream_t s;
+    if (!current_here(rd.dev, &s)) NOT_HERE;
+    const at::Tensor status = device_ints({m}, rd.dev);
+    const int rc = launch([&] {
+      return fn.fork_pages(&t, (const int32_t*)p->data_ptr(), (const int32_t*)c->data_ptr(), (int)m,
+                           (int32_t*)status.data_ptr(), s);
+    });
+    if (rc != 0) return failed(rc, "pa_fp8_fork_pages");
+    return THPVariable_Wrap(status);
+  });
+}
+
+// free_pages(block_tables, context_lengths, ref_counts, sequences, block_size, new_lengths) -> status
+PyObject* free_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 6) NOT_HERE;
+  return guarded([&]() -> PyObject* {
+    Reader rd;
+    pa_fp8_page_table_args t;
+    int64_t m = -1;
+    if (!read_table(a[0], a[1], a[2], a[4], rd, &t)) NOT_HERE;
+    const at::Tensor* q = rd(a[3]);
+    const at::Tensor* l = a[5] == Py_None ? nullptr : rd(a[5]);
+    if (!rd.ok || !int_list(q, 65536, &m) || (l && !int_list(l, 65536, &m))) NOT_HERE;
+    hipStream_t s;
+    if (!current_here(rd.dev, &s)) NOT_HERE;
+    const at::Tensor status = device_ints({m}, rd.dev);
+    const int rc = launch([&] {
+      return fn.free_pages(&t, (const int32_t*)q->data_ptr(), l ? (const int32_t*)l->data_ptr() : nullptr, (int)m,
+                           (int32_t*)status.data_ptr(), s);
+    });
+    if (rc != 0) return failed(rc, "pa_fp8_free_pages");
+    return THPVariable_Wrap(status);
+  });
+}
+
+// extend_pages(caches, block_tables, context_lengths, ref_counts, sequences, new_lengths, block_size) -> status
+PyObject* extend_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 7) NOT_HERE;
+  return guarded([&]() -> PyObject* {
+    Reader rd;
+    pa_fp8_page_table_args t;
+    std::vector<pa_fp8_page_cache> caches;
+    int64_t m = -1;
+    if (!read_table(a[1], a[2], a[3], a[6], rd, &t)) NOT_HERE;
+    const at::Tensor *q = rd(a[4]), *l = rd(a[5]);
+    if (!rd.ok || !int_list(q, 4096, &m) || !int_list(l, 4096, &m)) NOT_HERE;
+    int64_t pages = t.num_blocks;
+    if (!read_caches(a[0], rd, &pages, &caches)) NOT_HERE;
+    hipStream_t s;
+    if (!current_here(rd.dev, &s)) NOT_HERE;
+    const int64_t bytes = fn.pages_bytes(PA_PAGES_EXTEND, t.num_blocks, (int)m);
+    if (bytes < 0) NOT_HERE;
+    const at::Tensor status = device_ints({m}, rd.dev), ws = device_bytes(bytes, rd.dev);
+    const int rc = launch([&] {
+      return fn.extend_pages(&t, caches.data(), (int)caches.size(), (const int32_t*)q->data_ptr(),
+                             (const int32_t*)l->data_ptr(), (int)m, (int32_t*)status.data_ptr(), ws.data_ptr(), bytes, s);
+    });
+    if (rc != 0) return failed(rc, "pa_fp8_extend_pages");
+    return THPVariable_Wrap(status);
+  });
+}
+
+// compact_pages(caches, block_tables, context_lengths, ref_counts, block_size) -> (tables, counts, page map, live)
+PyObject* compact_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 5) NOT_HERE;
+  return guarded([&]() -> PyObject* {
+    Reader rd;
+    pa_fp8_page_table_args t;
+    std::vector<pa_fp8_page_cache> caches;
+    if (!read_table(a[1], a[2], a[3], a[4], rd, &t)) NOT_HERE;
+    int64_t pages = t.num_blocks;
+    if (!read_caches(a[0], rd, &pages, &caches)) NOT_HERE;
+    hipStream_t s;
+    if (!current_here(rd.dev, &s)) NOT_HERE;
+    const int64_t bytes = fn.pages_bytes(PA_PAGES_COMPACT, t.num_blocks, 0);
+    if (bytes < 0) NOT_HERE;
+    const at::Tensor tables = device_ints({t.num_rows, t.max_blocks_per_seq}, rd.dev),
+                     counts = device_ints({t.num_blocks}, rd.dev), map = device_ints({t.num_blocks}, rd.dev),
+                     live = device_ints({1}, rd.dev), ws = device_bytes(bytes, rd.dev);
+    const int rc = launch([&] {
+      return fn.compact_pages(&t, caches.data(), (int)caches.size(), (int32_t*)tables.data_ptr(), tables.stride(0),
+                              (int32_t*)counts.data_ptr(), (int32_t*)map.data_ptr(), (int32_t*)live.data_ptr(),
+                              ws.data_ptr(), bytes, s);
+    });
+    if (rc != 0) return failed(rc, "pa_fp8_compact_pages");
+    PyObject* out = PyTuple_New(4);
+    if (!out) return nullptr;
+    PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(tables));
+    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(counts));
+    PyTuple_SET_ITEM(out, 2, THPVariable_Wrap(map));
+    PyTuple_SET_ITEM(out, 3, THPVariable_Wrap(live));
+    return out;
+  });
+}
+
 // init(addresses in the order of Entry's fields, check): the entry points of
 // the loaded library.
 PyObject* init(PyObject*, PyObject* args) {
@@ -808,6 +1133,12 @@ PyMethodDef methods[] = {
     {"qknr", (PyCFunction)(void (*)(void))qknr, METH_FASTCALL, nullptr},
     {"mla_decode", (PyCFunction)(void (*)(void))mla_decode, METH_FASTCALL, nullptr},
     {"mla_reduce", (PyCFunction)(void (*)(void))mla_reduce, METH_FASTCALL, nullptr},
+    {"shared_prefix", (PyCFunction)(void (*)(void))shared_prefix, METH_FASTCALL, nullptr},
+    {"copy_pages", (PyCFunction)(void (*)(void))copy_pages, METH_FASTCALL, nullptr},
+    {"fork_pages", (PyCFunction)(void (*)(void))fork_pages, METH_FASTCALL, nullptr},
+    {"extend_pages", (PyCFunction)(void (*)(void))extend_pages, METH_FASTCALL, nullptr},
+    {"free_pages", (PyCFunction)(void (*)(void))free_pages, METH_FASTCALL, nullptr},
+    {"compact_pages", (PyCFunction)(void (*)(void))compact_pages, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -52,3 +52,4 @@ int pa_violations_mla(unsigned int* bits);
 int pa_violations_rope_cache(unsigned int* bits);
 int pa_violations_qk_norm_rope(unsigned int* bits);
 int pa_violations_shared_prefix(unsigned int* bits);
+int pa_violations_cache_pages(unsigned int* bits);

@@ -4986,6 +4986,7 @@ int pa_fp8_debug_violations(unsigned int* bits) {
   if (rc == 0) rc = pa_violations_rope_cache(bits);
   if (rc == 0) rc = pa_violations_qk_norm_rope(bits);
   if (rc == 0) rc = pa_violations_shared_prefix(bits);
+  if (rc == 0) rc = pa_violations_cache_pages(bits);
   return rc;
 }
 

@@ -101,6 +101,11 @@ def pa_decode_shared_prefix(
     group size, up to 4096 sequences and 1024 groups.  Returns the route name.
     Under graph capture the scales must be float32 device tensors.
     """
+    native = _lib.native()
+    if native is not None and stream is None and native.shared_prefix(
+            output, query, key_cache, value_cache, context_lengths, block_tables, prefix_indptr, prefix_lengths,
+            softmax_scale, key_scale, value_scale, _cu_count):
+        return ROUTE
     return prepare_pa_decode_shared_prefix(
         output, query, key_cache, value_cache, context_lengths, block_tables, prefix_indptr, prefix_lengths,
         softmax_scale, key_scale, value_scale, stream=stream).launch()

@@ -689,6 +689,78 @@ int pa_fp8_plan_shared_prefix(const int32_t* context_lengths, const int32_t* pre
                               int max_pieces, int32_t* pieces);
 
 /*
+ * Page operators of a paged cache.  No counterpart in the reference.
+ *
+ * State: block tables [num_rows, max_blocks_per_seq] (a row of num_rows holds
+ * one sequence, of context_lengths[row] tokens; 0: none), and one reference
+ * count a page, 0 where the page is free.  Caches: any number of tensors whose
+ * first dimension is the page; a page's page_bytes lie together, stride_bytes
+ * apart.  The page size is any power of two up to 2^20 tokens.
+ *
+ * Every operator decides on the state as it was before the call.  Lists name
+ * rows (or pages); entry i's status is 1 where it was carried out and 0 where
+ * it was left out: a row, page or length out of range, or a rule below.  Table
+ * entries outside the cache are passed over.
+ *   copy:    page dst[i] := page src[i] in every cache.  Left out where a later
+ *            entry has the same target, or the target is another entry's
+ *            source.  At most 65536 entries.
+ *   fork:    row children[i], which must be empty (length 0), gets the pages and
+ *            the length of row parents[i], and each page one more holder.  Left
+ *            out where an earlier entry has the child, or the parent is itself
+ *            a child in the list.  At most 65536 entries.
+ *   extend:  row sequences[i] grows to new_lengths[i] tokens (at least its
+ *            length): free pages, lowest first, in the order of the list; a last
+ *            page that is part full and has other holders is replaced by a copy,
+ *            unless all of the others are listed earlier.  Left out where an
+ *            earlier entry has the row; once the pool is short of an entry, it
+ *            and all behind it are left out.  At most 4096 entries.
+ *   free:    row sequences[i] keeps new_lengths[i] tokens (NULL: 0; at most its
+ *            length), and the pages behind lose a holder.  Left out where an
+ *            earlier entry has the row.  At most 65536 entries.
+ *   compact: with `live` pages held, the k-th held page at or above index `live`
+ *            moves to the k-th free page below it, in every cache.  Writes new
+ *            tables, new counts, page_map [num_blocks] (a page's new index, -1
+ *            where it was free) and live [1]; the old state and every held page
+ *            stay as they were, so that work on them may still run.
+ * Pools of at most 4 Mi pages.  Workspaces (pa_fp8_pages_workspace_bytes) need
+ * no initialisation and belong to the call until its launches end.
+ */
+typedef struct pa_fp8_page_table_args {
+  int32_t abi_version; /* = PA_FP8_ABI_VERSION */
+  int32_t* block_tables;
+  int32_t* context_lengths;
+  int32_t* ref_counts;
+  int64_t stride_bt_seq;
+  int32_t num_rows;
+  int32_t max_blocks_per_seq;
+  int32_t num_blocks;
+  int32_t block_size;
+} pa_fp8_page_table_args;
+
+typedef struct pa_fp8_page_cache {
+  void* data;
+  int64_t stride_bytes;
+  int64_t page_bytes;
+} pa_fp8_page_cache;
+
+enum { PA_PAGES_COPY = 0, PA_PAGES_EXTEND = 1, PA_PAGES_COMPACT = 2 };
+/* n: entries of the list (compact: 0). */
+int64_t pa_fp8_pages_workspace_bytes(int operation, int num_blocks, int n);
+int pa_fp8_copy_pages(const pa_fp8_page_cache* caches, int num_caches, int num_blocks, const int32_t* src,
+                      const int32_t* dst, int n, int32_t* status, void* workspace, int64_t workspace_bytes,
+                      void* hip_stream);
+int pa_fp8_fork_pages(const pa_fp8_page_table_args* table, const int32_t* parents, const int32_t* children, int n,
+                      int32_t* status, void* hip_stream);
+int pa_fp8_extend_pages(const pa_fp8_page_table_args* table, const pa_fp8_page_cache* caches, int num_caches,
+                        const int32_t* sequences, const int32_t* new_lengths, int n, int32_t* status, void* workspace,
+                        int64_t workspace_bytes, void* hip_stream);
+int pa_fp8_free_pages(const pa_fp8_page_table_args* table, const int32_t* sequences, const int32_t* new_lengths, int n,
+                      int32_t* status, void* hip_stream);
+int pa_fp8_compact_pages(const pa_fp8_page_table_args* table, const pa_fp8_page_cache* caches, int num_caches,
+                         int32_t* new_tables, int64_t stride_new_tables, int32_t* new_ref_counts, int32_t* page_map,
+                         int32_t* live, void* workspace, int64_t workspace_bytes, void* hip_stream);
+
+/*
  * Checked builds.  libpa_fp8_checked.so is built from the same sources with
  * -DPA_FP8_CHECKED.  Like the release library it clamps every index it reads
  * from caller data into range before using it as an address; it also
@@ -696,7 +768,8 @@ int pa_fp8_plan_shared_prefix(const int32_t* context_lengths, const int32_t* pre
  * wait; the results are those of the release library):
  */
 enum {
-  PA_VIOLATION_PAGE = 1,     /* block_tables / kv_page_indices entry, or fnuz row index, outside the cache */
+  PA_VIOLATION_PAGE = 1,     /* block_tables / kv_page_indices entry, page of a copy, or fnuz row index, outside the
+                              * cache; a page freed more often than it was held */
   PA_VIOLATION_WORK = 2,     /* MLA work record: query row, partial row or kv range outside its buffer */
   PA_VIOLATION_POSITION = 4, /* rope position outside [0, max_pos) */
   PA_VIOLATION_SLOT = 8      /* KV-cache slot past the last cache block */
