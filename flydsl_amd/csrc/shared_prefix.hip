@@ -7,24 +7,31 @@
 //   out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i,   M = max m_i
 //
 // Work decomposition: see sp_plan.h.  One launch of persistent workgroups
-// (eight waves) walks equal shares of the line of prefix and suffix items and
-// leaves float32 pieces; a second launch merges a row's pieces.
+// (four waves, two workgroups a CU) walks equal shares of the line of prefix
+// and suffix items and leaves float32 pieces; a second launch merges a row's
+// pieces.
 //
 // Arithmetic.  A wave holds NR tiles of 16 query rows and walks 64-token
 // tiles.  Keys and values are fp8 e4m3fn, exact in bf16 and f16, so they are
 // converted and both products run on v_mfma_f32_16x16x32_{bf16,f16}:
-//   S^T = K Q^T   A: 16 tokens x 32 dims, B: Q^T
+//   S^T = K Q^T     A: 16 tokens x 32 dims, B: Q^T
 //   O^T += V^T P^T  A: 16 dims x 32 tokens, B: P^T
-// Lane (c, g) = (l % 16, l / 16) loads 16-byte pieces straight from the
-// cache's layout: of keys, 16 dims of one token (the k order of S is a
-// permutation of the head dimension that Q shares); of values, the 16 tokens
-// of block g for one dim.  Row m of key tile T is token 16 (m / 4) + 4 T +
-// m % 4, so that the logits lane (c, g) gets from the four tiles are those of
-// row c and the 16 tokens of block g -- the very tokens its value operand
-// holds, and the probabilities need no move between lanes.
+// Row m of key tile T (of four) is token 16 (m / 4) + 4 T + m % 4, so that the
+// logits that lane (c, g) = (l % 16, l / 16) gets are those of row c and the
+// tokens 16 g + 4 T .. + 3: with all four tiles, or with T = 2 j and 2 j + 1, the
+// very tokens 16 g + 8 j .. + 7 that the lane supplies to value product j, and
+// the probabilities need no move between lanes.
 // The probabilities are rounded to the operands' type, by at most 2^-8 (bf16)
 // or 2^-11 (f16) of themselves, as an attention in that type rounds them;
 // sums, maxima and outputs stay in 32 bits.
+//
+// Few rows (run_direct): bound by HBM; a wave's 16-byte loads bring keys (16
+// dims of a token; the k order of S is a permutation of the head dimension
+// that Q shares) and values (the 16 tokens of block g for one dim) straight
+// from the cache's layout into operand registers.
+// Many rows (run_shared): bound by the matrix cores, the vector units and LDS
+// alike; the workgroup converts each tile once, into LDS in the operands' order,
+// while the tile before is computed (two buffers, one barrier a tile).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -195,13 +202,13 @@ __device__ void block_scan(T* a, int n, int64_t* scratch) {
   __syncthreads();
 }
 
-// Last entry of a[0 .. n] (never falls) that is <= x, for a[0] <= x.
+// Last entry of a[0 .. n] (never falls) that, times k, is <= x, for a[0] = 0 or <= x.
 template <typename T>
-__device__ __forceinline__ int last_le(const T* a, int n, int64_t x) {
+__device__ __forceinline__ int last_le(const T* a, int n, int64_t x, int k = 1) {
   int lo = 0, hi = n + 1;
   while (hi - lo > 1) {
     const int m = (lo + hi) >> 1;
-    if ((int64_t)a[m] <= x)
+    if (k * (int64_t)a[m] <= x)
       lo = m;
     else
       hi = m;
@@ -231,7 +238,7 @@ __device__ void make_plan(const Plan& p, const SpArgs& s) {
       const int tiles = len > 0 ? pa_cdiv(rows, s.p.rows) : 0;
       p.len[g] = len;
       p.row_tiles[g] = tiles;
-      p.group_at[g] = (int64_t)tiles * sp_item_cost(sp_steps(0, len, s.p.wt), s.p.cost);
+      p.group_at[g] = (int64_t)tiles * sp_item_cost(sp_steps(0, len, s.p.tiles), s.p.cost);
     }
     block_scan<false>(p.row_tiles, G, p.scratch);
     block_scan<false>(p.group_at, G, p.scratch);
@@ -241,7 +248,7 @@ __device__ void make_plan(const Plan& p, const SpArgs& s) {
   for (int b = threadIdx.x; b < B; b += kThreads) {
     const int g = group_of(p, G, b);
     const int len = g >= 0 ? p.len[g] : 0;
-    p.seq_at[b] = (int64_t)s.col_tiles * sp_item_cost(sp_steps(len, context_of(s, b), s.s.wt), s.s.cost);
+    p.seq_at[b] = (int64_t)s.col_tiles * sp_item_cost(sp_steps(len, context_of(s, b), s.s.tiles), s.s.cost);
   }
   block_scan<false>(p.seq_at, B, p.scratch);
 }
@@ -251,83 +258,202 @@ __device__ void make_plan(const Plan& p, const SpArgs& s) {
 // ---------------------------------------------------------------------------
 
 struct Piece {
-  bool prefix;
   int b0;            // sequence whose table row gives the pages, and of the item's row 0
   int row0, nrows;   // first row of the item among the group's rows (the sequence's columns), and their count
   int h;             // kv head
   int begin, end;    // tokens of the item
   int tile, tile_end;  // tiles of the piece
-  int wt, waves_r, rows_out;
+  int rows_out;      // rows of a slot
   float* ml;         // the slot
   float* o;
 };
 
-// LDS of the pieces' ends: maxima and sums by wave, then 32 output dims.
+// LDS behind the plan: two buffers of a tile's keys and values in 16 bits and
+// their scales, or, at a piece's end, maxima and sums by wave and 32 output
+// dims of every row.
 constexpr int kOutStride = 36;  // floats a row of 32 dims takes (16-byte steps that spread over the banks)
 __host__ __device__ constexpr int end_bytes(int nr) {
   return SP_WAVES * 16 * nr * 4 * 2 + SP_WAVES * 16 * nr * kOutStride * 4;
 }
+__host__ __device__ constexpr int tile_bytes(int d) { return 2 * SP_TILE * d * 2; }
+__host__ __device__ constexpr int work_bytes(int d, bool shared) {
+  return shared ? 2 * (tile_bytes(d) + 2 * SP_TILE * 4) : end_bytes(d <= 128 ? 2 : 1);
+}
 
-template <int D, bool F16, bool PT, int NR>
-__device__ __forceinline__ void run_piece(const SpArgs& s, const Piece& pc, char* lds) {
+// The wave's rows: operand B of the key product, the keys each row sees, and
+// their softmax.
+template <int D, int NR>
+struct Rows {
+  i32x4 q[NR][D / 32];
+  f32x4 o[NR][D / 16];
+  float m[NR], l[NR];
+  int limit[NR];  // keys a row sees: below it
+  int least;      // of all of the wave's
+  float fac;      // of a raw logit, positive
+
+  // `wr`: which of the item's waves; DIMS16: a lane's k order is 16 dims of two
+  // steps (run_direct), else 8 of each.
+  template <bool DIMS16, bool PT>
+  __device__ __forceinline__ void load(const SpArgs& s, const Piece& pc, int wr, int c, int g) {
+    const pa_fp8_shared_prefix_args& a = s.a;
+    const int eq = s.eq, ql = a.query_length, gqa = a.query_group_size;
+    const float c0 = a.softmax_scale * kLog2e * (PT ? 1.0f : a.key_scale[0]);
+    fac = c0 == 0.0f ? 1.0f : fabsf(c0);
+    const int flip = c0 < 0.0f ? (int)0x80008000u : 0, keep = c0 == 0.0f ? 0 : -1;
+    least = 0x7fffffff;
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      const int r = pc.row0 + (wr * NR + n) * 16 + c;
+      const bool live = r < pc.nrows;
+      const int bb = live ? r / eq : 0, e = live ? r - bb * eq : 0;
+      const int b = pc.b0 + bb, qi = e / gqa;
+      limit[n] = 0x7fffffff;
+      if (live) limit[n] = pa_min(pa_max(a.context_lengths[b] - ql + qi + 1, 0), pc.end);
+      least = pa_min(least, limit[n]);
+      const uint16_t* row = (const uint16_t*)a.query + (int64_t)(b * (int64_t)ql + qi) * a.stride_q_tok +
+                            (int64_t)(pc.h * gqa + (e - qi * gqa)) * a.stride_q_head;
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) {
+        i32x4 w = {0, 0, 0, 0};
+        if (live) w = *(const i32x4*)(row + (DIMS16 ? (4 * (k >> 1) + g) * 16 + 8 * (k & 1) : 32 * k + 8 * g));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (w[i] ^ flip) & keep;
+        q[n][k] = w;
+      }
+      m[n] = kNegInf;
+      l[n] = 0.0f;
+#pragma unroll
+      for (int dt = 0; dt < D / 16; ++dt) o[n][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) least = pa_min(least, __shfl_xor(least, d, 64));
+    least = __builtin_amdgcn_readfirstlane(least);
+  }
+
+  // Softmax of NT tiles' logits x (tokens t0 + 16 g + 4 (T0 + T) + i of the lane's
+  // row n) against the row's reference; p: the probabilities (times vs) as
+  // operands.
+  template <bool PT, bool PF16, int NT>
+  __device__ __forceinline__ void softmax(int n, const f32x4 (&x)[NT], const f32x4 (&vs)[NT], i32x4 (&p)[NT / 2]) {
+    float top = kNegInf;
+#pragma unroll
+    for (int T = 0; T < NT; ++T)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, x[T][i]);
+    top = groups_max(top) * fac;
+    if (__ballot(top > m[n] + kRescaleMargin)) {
+      const float mn = fmaxf(m[n], top);
+      const float f = mn == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m[n] - mn);
+      l[n] *= f;
+#pragma unroll
+      for (int dt = 0; dt < D / 16; ++dt) o[n][dt] *= f;
+      m[n] = mn;
+    }
+    const float bias = m[n] == kNegInf ? 0.0f : -m[n];
+    float w[4 * NT], sum = 0.0f;
+#pragma unroll
+    for (int T = 0; T < NT; ++T)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[T][i], fac, bias));
+        sum += e;
+        w[4 * T + i] = PT ? e * vs[T][i] : e;
+      }
+    l[n] += sum;
+#pragma unroll
+    for (int j = 0; j < NT / 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[j][i] = round2<PF16>(w[8 * j + 2 * i], w[8 * j + 2 * i + 1]);
+  }
+
+  // Joins the waves of the same rows (wt of them, this one the wi-th) and writes
+  // the piece.
+  __device__ __forceinline__ void finish(const Piece& pc, char* lds, int wt, int wave, int wr, int wi, int c, int g) {
+    float* lm = (float*)lds;              // [wave][16 NR]
+    float* ll = lm + SP_WAVES * 16 * NR;
+    float* lo = ll + SP_WAVES * 16 * NR;  // [wave][16 NR][kOutStride]
+    __syncthreads();                      // what LDS held before has been read
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      l[n] = groups_sum(l[n]);
+      if (g == 0) {
+        lm[(wave * NR + n) * 16 + c] = m[n];
+        ll[(wave * NR + n) * 16 + c] = l[n];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      float top = kNegInf, sum = 0.0f;
+      for (int w = wr * wt; w < (wr + 1) * wt; ++w) top = fmaxf(top, lm[(w * NR + n) * 16 + c]);
+      for (int w = wr * wt; w < (wr + 1) * wt; ++w) {
+        const float mw = lm[(w * NR + n) * 16 + c];
+        // (a wave that saw no key has 0 or, where its logits were NaN, NaN)
+        sum += ll[(w * NR + n) * 16 + c] * (mw == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mw - top));
+      }
+      const float f = m[n] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m[n] - top);
+#pragma unroll
+      for (int dt = 0; dt < D / 16; ++dt) o[n][dt] *= f;
+      const int r = (wr * NR + n) * 16 + c;
+      if (wi == 0 && g == 0 && pc.row0 + r < pc.nrows) {
+        pc.ml[r] = top;
+        pc.ml[pc.rows_out + r] = sum;
+      }
+    }
+    const int rows = SP_WAVES / wt * 16 * NR;
+#pragma unroll
+    for (int d0 = 0; d0 < D / 32; ++d0) {
+      if (d0) __syncthreads();
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          *(f32x4*)(lo + ((wave * NR + n) * 16 + c) * kOutStride + 16 * k + 4 * g) = o[n][2 * d0 + k];
+      __syncthreads();
+      for (int i = threadIdx.x; i < rows * 8; i += kThreads) {
+        const int r = i >> 3, d = (i & 7) * 4;
+        if (pc.row0 + r >= pc.nrows) break;  // (rows only grow with i)
+        const int w0 = r / (16 * NR) * wt, rr = r % (16 * NR);
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+        for (int w = w0; w < w0 + wt; ++w) sum += *(const f32x4*)(lo + (w * 16 * NR + rr) * kOutStride + d);
+        *(f32x4*)(pc.o + (int64_t)r * D + 32 * d0 + d) = sum;
+      }
+    }
+    __syncthreads();  // LDS is the next piece's
+  }
+};
+
+// The item's pages: of a token, inside the cache and the table row whatever
+// the caller's table holds.
+struct Pages {
+  const int32_t* table;
+  int last, lbs, blocks;
+  __device__ __forceinline__ Pages(const SpArgs& s, const Piece& pc)
+      : table(s.a.block_tables + (int64_t)pc.b0 * s.a.stride_bt_seq),
+        last(pa_min((pc.end - 1) >> s.lbs, s.a.max_blocks_per_seq - 1)),
+        lbs(s.lbs),
+        blocks(s.a.num_blocks) {}
+  __device__ __forceinline__ int operator()(int token) const {
+    int p = table[pa_min(token >> lbs, last)];
+    pa_note(p < 0 || p >= blocks, PA_VIOLATION_PAGE);
+    p = p < 0 ? 0 : p;
+    return p < blocks ? p : blocks - 1;
+  }
+};
+
+template <int D, bool F16, bool PT>
+__device__ __forceinline__ void run_direct(const SpArgs& s, const Piece& pc, char* lds) {
   // the value product of f16 queries with per-token scales runs in bf16: a
   // scale of any size times a probability stays in range
   constexpr bool PF16 = F16 && !PT;
   const pa_fp8_shared_prefix_args& a = s.a;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wr = wave / pc.wt, wi = wave - wr * pc.wt;
-  const int eq = s.eq, ql = a.query_length, gqa = a.query_group_size;
   const int bs = 1 << s.lbs;
-
-  // ---- query rows ----
-  const float c0 = a.softmax_scale * kLog2e * (PT ? 1.0f : a.key_scale[0]);
-  const float fac = c0 == 0.0f ? 1.0f : fabsf(c0);
-  const int flip = c0 < 0.0f ? (int)0x80008000u : 0, keep = c0 == 0.0f ? 0 : -1;
-  i32x4 q[NR][D / 32];
-  int limit[NR];  // keys the row sees: below it
-  int least = 0x7fffffff;
-#pragma unroll
-  for (int n = 0; n < NR; ++n) {
-    const int r = pc.row0 + (wr * NR + n) * 16 + c;
-    const bool live = r < pc.nrows;
-    const int bb = live ? r / eq : 0, e = live ? r - bb * eq : 0;
-    const int b = pc.b0 + bb, qi = e / gqa;
-    limit[n] = 0x7fffffff;
-    if (live) {
-      const int ctx = a.context_lengths[b];
-      limit[n] = pa_min(pa_max(ctx - ql + qi + 1, 0), pc.end);
-    }
-    least = pa_min(least, limit[n]);
-    const uint16_t* row = (const uint16_t*)a.query + (int64_t)(b * (int64_t)ql + qi) * a.stride_q_tok +
-                          (int64_t)(pc.h * gqa + (e - qi * gqa)) * a.stride_q_head;
-#pragma unroll
-    for (int u = 0; u < D / 64; ++u)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        i32x4 w = {0, 0, 0, 0};
-        if (live) w = *(const i32x4*)(row + (4 * u + g) * 16 + 8 * k);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = (w[i] ^ flip) & keep;
-        q[n][2 * u + k] = w;
-      }
-  }
-#pragma unroll
-  for (int d = 1; d < 16; d *= 2) least = pa_min(least, __shfl_xor(least, d, 64));
-  least = __builtin_amdgcn_readfirstlane(least);
-
-  // ---- addresses ----
-  const int32_t* table = a.block_tables + (int64_t)pc.b0 * a.stride_bt_seq;
-  const int last_page = pa_min((pc.end - 1) >> s.lbs, a.max_blocks_per_seq - 1);
+  const Pages page_of(s, pc);
   const uint8_t* kbase = (const uint8_t*)a.key_cache + (int64_t)pc.h * a.stride_k_head;
   const uint8_t* vbase = (const uint8_t*)a.value_cache + (int64_t)pc.h * a.stride_v_head;
   const int v_dim = a.trans_v ? 16 : bs, v_blk = a.trans_v ? D * 16 : 16;
-  auto page_of = [&](int token) -> int {
-    int p = table[pa_min(token >> s.lbs, last_page)];
-    pa_note(p < 0 || p >= a.num_blocks, PA_VIOLATION_PAGE);
-    p = p < 0 ? 0 : p;
-    return p < a.num_blocks ? p : a.num_blocks - 1;
-  };
   const int kblk = c >> 2;  // the lane's key tokens are of block kblk, its value tokens of block g
   i32x4 kr[4][D / 64], vr[D / 16];
   f32x4 ks[4], vs[4];
@@ -352,75 +478,62 @@ __device__ __forceinline__ void run_piece(const SpArgs& s, const Piece& pc, char
     for (int T = 0; T < 4; ++T) x[T] = *(const f32x4*)(p + 4 * T);
   };
 
-  f32x4 o[NR][D / 16];
-  float m[NR], l[NR];
-#pragma unroll
-  for (int n = 0; n < NR; ++n) {
-    m[n] = kNegInf;
-    l[n] = 0.0f;
-#pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt) o[n][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-
-  int tile = pc.tile + wi;
+  int tile = pc.tile + wave;
   int kp = 0, vp = 0;
   if (tile < pc.tile_end) {
     kp = page_of(tile * SP_TILE + 16 * kblk);
     vp = page_of(tile * SP_TILE + 16 * g);
+  }
+  Rows<D, 1> w;
+  w.template load<true, PT>(s, pc, 0, c, g);
+  if (tile < pc.tile_end) {
     load_keys(tile, kp);
     load_values(tile, vp);
     if constexpr (PT) {
       load_scales(a.key_scale, tile, vp, ks);
       load_scales(a.value_scale, tile, vp, vs);
     }
-    const int next = pa_min(tile + pc.wt, pc.tile_end - 1);
+    const int next = pa_min(tile + SP_WAVES, pc.tile_end - 1);
     kp = page_of(next * SP_TILE + 16 * kblk);
     vp = page_of(next * SP_TILE + 16 * g);
   }
-  for (; tile < pc.tile_end; tile += pc.wt) {
-    const int next = tile + pc.wt;
+  for (; tile < pc.tile_end; tile += SP_WAVES) {
+    const int next = tile + SP_WAVES;
     const bool more = next < pc.tile_end;
-    // ---- logits of tokens 16 g + 4 T + i ----
-    f32x4 x[NR][4];
+    f32x4 x[4];
 #pragma unroll
     for (int T = 0; T < 4; ++T) {
-#pragma unroll
-      for (int n = 0; n < NR; ++n) x[n][T] = f32x4{0.f, 0.f, 0.f, 0.f};
+      x[T] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int u = 0; u < D / 64; ++u) {
         const i32x4 k0 = widen8<F16>(kr[T][u][0], kr[T][u][1]), k1 = widen8<F16>(kr[T][u][2], kr[T][u][3]);
-#pragma unroll
-        for (int n = 0; n < NR; ++n) {
-          x[n][T] = mfma<F16>(k0, q[n][2 * u], x[n][T]);
-          x[n][T] = mfma<F16>(k1, q[n][2 * u + 1], x[n][T]);
-        }
+        x[T] = mfma<F16>(k0, w.q[0][2 * u], x[T]);
+        x[T] = mfma<F16>(k1, w.q[0][2 * u + 1], x[T]);
       }
     }
     if (more) load_keys(next, kp);
     if constexpr (PT) {
 #pragma unroll
-      for (int n = 0; n < NR; ++n)
-#pragma unroll
-        for (int T = 0; T < 4; ++T) x[n][T] *= ks[T];
+      for (int T = 0; T < 4; ++T) x[T] *= ks[T];
       if (more) load_scales(a.key_scale, next, vp, ks);
     }
     // ---- masks: the part's first and last tiles ----
     const int t0 = tile * SP_TILE;
-    if (t0 < pc.begin || t0 + SP_TILE > pa_min(least, pc.end)) {
+    if (t0 < pc.begin || t0 + SP_TILE > pa_min(w.least, pc.end)) {
 #pragma unroll
-      for (int n = 0; n < NR; ++n)
+      for (int T = 0; T < 4; ++T)
 #pragma unroll
-        for (int T = 0; T < 4; ++T)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int t = t0 + 16 * g + 4 * T + i;
-            if (t < pc.begin || t >= limit[n]) x[n][T][i] = kNegInf;
-          }
+        for (int i = 0; i < 4; ++i) {
+          const int t = t0 + 16 * g + 4 * T + i;
+          if (t < pc.begin || t >= w.limit[0]) x[T][i] = kNegInf;
+        }
       // bytes behind the part's tokens may be anything, NaN among it
 #pragma unroll
-      for (int dt = 0; dt < D / 16; ++dt)
+      for (int i = 0; i < 4; ++i) {
+        const int keep = (int)keep4(t0 + 16 * g + 4 * i, pc.begin, pc.end);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) vr[dt][i] &= (int)keep4(t0 + 16 * g + 4 * i, pc.begin, pc.end);
+        for (int dt = 0; dt < D / 16; ++dt) vr[dt][i] &= keep;
+      }
       if constexpr (PT) {
 #pragma unroll
         for (int T = 0; T < 4; ++T)
@@ -431,108 +544,187 @@ __device__ __forceinline__ void run_piece(const SpArgs& s, const Piece& pc, char
           }
       }
     }
-    // ---- softmax ----
-    i32x4 p[NR][2];
-#pragma unroll
-    for (int n = 0; n < NR; ++n) {
-      float top = kNegInf;
-#pragma unroll
-      for (int T = 0; T < 4; ++T)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, x[n][T][i]);
-      top = groups_max(top) * fac;
-      if (__ballot(top > m[n] + kRescaleMargin)) {
-        const float mn = fmaxf(m[n], top);
-        const float f = mn == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m[n] - mn);
-        l[n] *= f;
-#pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) o[n][dt] *= f;
-        m[n] = mn;
-      }
-      const float bias = m[n] == kNegInf ? 0.0f : -m[n];
-      float w[16];
-#pragma unroll
-      for (int T = 0; T < 4; ++T)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][T][i], fac, bias));
-          l[n] += e;
-          w[4 * T + i] = PT ? e * vs[T][i] : e;
-        }
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[n][j][i] = round2<PF16>(w[8 * j + 2 * i], w[8 * j + 2 * i + 1]);
-    }
-    // ---- values ----
+    i32x4 p[2];
+    w.template softmax<PT, PF16, 4>(0, x, vs, p);
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) {
       const i32x4 v0 = widen8<PF16>(vr[dt][0], vr[dt][1]), v1 = widen8<PF16>(vr[dt][2], vr[dt][3]);
-#pragma unroll
-      for (int n = 0; n < NR; ++n) {
-        o[n][dt] = mfma<PF16>(v0, p[n][0], o[n][dt]);
-        o[n][dt] = mfma<PF16>(v1, p[n][1], o[n][dt]);
-      }
+      w.o[0][dt] = mfma<PF16>(v0, p[0], w.o[0][dt]);
+      w.o[0][dt] = mfma<PF16>(v1, p[1], w.o[0][dt]);
     }
     if (more) {
       load_values(next, vp);
       if constexpr (PT) load_scales(a.value_scale, next, vp, vs);
-      const int after = pa_min(next + pc.wt, pc.tile_end - 1);
+      const int after = pa_min(next + SP_WAVES, pc.tile_end - 1);
       kp = page_of(after * SP_TILE + 16 * kblk);
       vp = page_of(after * SP_TILE + 16 * g);
     }
   }
+  w.finish(pc, lds, SP_WAVES, wave, 0, wave, c, g);
+}
 
-  // ---- the waves of the same rows, merged; the piece written ----
-  float* lm = (float*)lds;                       // [wave][16 NR]
-  float* ll = lm + SP_WAVES * 16 * NR;
-  float* lo = ll + SP_WAVES * 16 * NR;           // [wave][16 NR][kOutStride]
-  __syncthreads();                               // the piece before has been read
+// A tile in LDS, 16-byte pieces: keys [D / 8 octets of dims][64 rows of the key
+// tiles], values [8 octets of tokens][D dims] -- an operand read takes 16
+// consecutive pieces a lane group, and so does a wave's write.
+template <int D, bool F16, bool PT, int NR, int WT>
+__device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, char* lds) {
+  constexpr bool PF16 = F16 && !PT;
+  constexpr int NT = 4 / WT, NJ = 2 / WT;  // the wave's key tiles and value products
+  constexpr int NS = D / 64;               // pieces of keys, and of values, that a thread brings
+  const pa_fp8_shared_prefix_args& a = s.a;
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wave / WT, wi = wave % WT;
+  const int bs = 1 << s.lbs;
+  const Pages page_of(s, pc);
+  const uint8_t* kbase = (const uint8_t*)a.key_cache + (int64_t)pc.h * a.stride_k_head;
+  const uint8_t* vbase = (const uint8_t*)a.value_cache + (int64_t)pc.h * a.stride_v_head;
+  const int v_dim = a.trans_v ? 16 : bs, v_blk = a.trans_v ? D * 16 : 16;
+  const float* ks_base = (threadIdx.x < SP_TILE ? a.key_scale : a.value_scale) + (int64_t)pc.h * a.stride_ks_head;
+
+  // what this thread brings: row `lane` of the key tiles, dims 16 (wave + 4 i); of
+  // piece threadIdx.x + 256 i of the values, its dim and token block
+  const int k_tok = 16 * ((lane & 15) >> 2) + 4 * (lane >> 4) + (lane & 3);
+  i32x4 kst[NS], vst[NS];
+  float sst = 0.0f;
+  int kpage, vpage[NS], spage = 0;
+  auto v_block = [&](int i) { return (int)(threadIdx.x + kThreads * i) / D; };
+  auto v_dim_of = [&](int i) { return (int)(threadIdx.x + kThreads * i) % D; };
+  auto pages = [&](int tile) {
+    kpage = page_of(tile * SP_TILE + (k_tok & ~15));
 #pragma unroll
-  for (int n = 0; n < NR; ++n) {
-    l[n] = groups_sum(l[n]);
-    if (g == 0) {
-      lm[(wave * NR + n) * 16 + c] = m[n];
-      ll[(wave * NR + n) * 16 + c] = l[n];
+    for (int i = 0; i < NS; ++i) vpage[i] = page_of(tile * SP_TILE + 16 * v_block(i));
+    if constexpr (PT) spage = page_of(tile * SP_TILE + (int)(threadIdx.x & (SP_TILE - 1)));
+  };
+  auto fetch = [&](int tile) {
+    const uint8_t* kp = kbase + (int64_t)kpage * a.stride_k_block + ((tile * SP_TILE + k_tok) & (bs - 1)) * 16;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) kst[i] = *(const i32x4*)(kp + (int64_t)(wave + SP_WAVES * i) * (bs * 16));
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const int in = ((tile * SP_TILE + 16 * v_block(i)) & (bs - 1)) >> 4;
+      vst[i] = *(const i32x4*)(vbase + (int64_t)vpage[i] * a.stride_v_block + in * v_blk + (int64_t)v_dim_of(i) * v_dim);
     }
-  }
+    if constexpr (PT) {
+      if (threadIdx.x < 2 * SP_TILE)
+        sst = ks_base[(int64_t)spage * a.stride_ks_block + ((tile * SP_TILE + (int)(threadIdx.x & (SP_TILE - 1))) & (bs - 1))];
+    }
+  };
+  constexpr int kBuffer = tile_bytes(D) + 2 * SP_TILE * 4;
+  auto store = [&](int tile, int buffer) {
+    i32x4* lk = (i32x4*)(lds + buffer * kBuffer);
+    i32x4* lv = lk + SP_TILE * D / 8;
+    const int t0 = tile * SP_TILE;
+    if (t0 < pc.begin || t0 + SP_TILE > pc.end) {  // bytes outside the part may be anything, NaN among it
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) vst[i][k] &= (int)keep4(t0 + 16 * v_block(i) + 4 * k, pc.begin, pc.end);
+      if constexpr (PT) {
+        const int t = t0 + (int)(threadIdx.x & (SP_TILE - 1));
+        if (t < pc.begin || t >= pc.end) sst = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const int o8 = 2 * (wave + SP_WAVES * i);
+      lk[o8 * SP_TILE + lane] = widen8<F16>(kst[i][0], kst[i][1]);
+      lk[(o8 + 1) * SP_TILE + lane] = widen8<F16>(kst[i][2], kst[i][3]);
+    }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const int at = 2 * v_block(i) * D + v_dim_of(i);
+      lv[at] = widen8<PF16>(vst[i][0], vst[i][1]);
+      lv[at + D] = widen8<PF16>(vst[i][2], vst[i][3]);
+    }
+    if constexpr (PT) {
+      if (threadIdx.x < 2 * SP_TILE) ((float*)(lv + SP_TILE * D / 8))[threadIdx.x] = sst;
+    }
+  };
+
+  pages(pc.tile);
+  Rows<D, NR> w;
+  w.template load<false, PT>(s, pc, wr, c, g);
+  fetch(pc.tile);
+  pages(pa_min(pc.tile + 1, pc.tile_end - 1));
+  store(pc.tile, 0);
+  if (pc.tile + 1 < pc.tile_end) fetch(pc.tile + 1);
+  pages(pa_min(pc.tile + 2, pc.tile_end - 1));
   __syncthreads();
+  int buffer = 0;
+  for (int tile = pc.tile; tile < pc.tile_end; ++tile, buffer ^= 1) {
+    const i32x4* lk = (const i32x4*)(lds + buffer * kBuffer);
+    const i32x4* lv = lk + SP_TILE * D / 8;
+    const float* lsc = (const float*)(lv + SP_TILE * D / 8);
+    f32x4 x[NR][NT], vs[NT];
 #pragma unroll
-  for (int n = 0; n < NR; ++n) {
-    float top = kNegInf, sum = 0.0f;
-    for (int w = wr * pc.wt; w < (wr + 1) * pc.wt; ++w) top = fmaxf(top, lm[(w * NR + n) * 16 + c]);
-    for (int w = wr * pc.wt; w < (wr + 1) * pc.wt; ++w) {
-      const float mw = lm[(w * NR + n) * 16 + c];
-      sum += mw == kNegInf ? ll[(w * NR + n) * 16 + c] * 0.0f : ll[(w * NR + n) * 16 + c] * __builtin_amdgcn_exp2f(mw - top);
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int n = 0; n < NR; ++n) x[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) {
+        const i32x4 kf = lk[(4 * k + g) * SP_TILE + (wi * NT + t) * 16 + c];
+#pragma unroll
+        for (int n = 0; n < NR; ++n) x[n][t] = mfma<F16>(kf, w.q[n][k], x[n][t]);
+      }
     }
-    const float f = m[n] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m[n] - top);
+    if constexpr (PT) {
 #pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt) o[n][dt] *= f;
-    const int r = (wr * NR + n) * 16 + c;
-    if (wi == 0 && g == 0 && pc.row0 + r < pc.nrows) {
-      pc.ml[r] = top;
-      pc.ml[pc.rows_out + r] = sum;
+      for (int t = 0; t < NT; ++t) {
+        const f32x4 k4 = *(const f32x4*)(lsc + 16 * g + 4 * (wi * NT + t));
+        vs[t] = *(const f32x4*)(lsc + SP_TILE + 16 * g + 4 * (wi * NT + t));
+#pragma unroll
+        for (int n = 0; n < NR; ++n) x[n][t] *= k4;
+      }
     }
-  }
-  const int rows_wg = pc.waves_r * 16 * NR;
+    const int t0 = tile * SP_TILE;
+    if (t0 < pc.begin || t0 + SP_TILE > pa_min(w.least, pc.end)) {
 #pragma unroll
-  for (int d0 = 0; d0 < D / 32; ++d0) {
-    if (d0) __syncthreads();
+      for (int n = 0; n < NR; ++n)
 #pragma unroll
-    for (int n = 0; n < NR; ++n)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-        *(f32x4*)(lo + ((wave * NR + n) * 16 + c) * kOutStride + 16 * k + 4 * g) = o[n][2 * d0 + k];
+          for (int i = 0; i < 4; ++i) {
+            const int at = t0 + 16 * g + 4 * (wi * NT + t) + i;
+            if (at < pc.begin || at >= w.limit[n]) x[n][t][i] = kNegInf;
+          }
+    }
+    i32x4 p[NR][NJ];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) w.template softmax<PT, PF16, NT>(n, x[n], vs, p[n]);
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const i32x4 vf = lv[(2 * g + wi * NJ + j) * D + 16 * dt + c];
+#pragma unroll
+        for (int n = 0; n < NR; ++n) w.o[n][dt] = mfma<PF16>(vf, p[n][j], w.o[n][dt]);
+      }
+    if (tile + 1 < pc.tile_end) {
+      store(tile + 1, buffer ^ 1);
+      if (tile + 2 < pc.tile_end) fetch(tile + 2);
+      pages(pa_min(tile + 3, pc.tile_end - 1));
+    }
     __syncthreads();
-    for (int i = threadIdx.x; i < rows_wg * 8; i += kThreads) {
-      const int r = i >> 3, d = (i & 7) * 4;
-      if (pc.row0 + r >= pc.nrows) break;  // (rows only grow with i)
-      const int w0 = r / (16 * NR) * pc.wt, rr = r % (16 * NR);
-      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-      for (int w = w0; w < w0 + pc.wt; ++w) sum += *(const f32x4*)(lo + (w * 16 * NR + rr) * kOutStride + d);
-      *(f32x4*)(pc.o + (int64_t)r * D + 32 * d0 + d) = sum;
+  }
+  w.finish(pc, lds, WT, wave, wr, wi, c, g);
+}
+
+template <int D, bool F16, bool PT>
+__device__ __forceinline__ void run_piece(const SpArgs& s, const SpShape& sh, const Piece& pc, char* lds) {
+  constexpr int most = D <= 128 ? 2 : 1;
+  if constexpr (D <= 128) {
+    if (!sh.shared) {
+      run_direct<D, F16, PT>(s, pc, lds);
+      return;
     }
   }
+  if (sh.wt == 1)
+    run_shared<D, F16, PT, most, 1>(s, pc, lds);
+  else if (most == 1 || sh.nr == 1)
+    run_shared<D, F16, PT, 1, 2>(s, pc, lds);
+  else
+    run_shared<D, F16, PT, most, 2>(s, pc, lds);
 }
 
 // ---------------------------------------------------------------------------
@@ -562,99 +754,80 @@ __global__ __launch_bounds__(kThreads, 2) void pa_shared_prefix_kernel(const SpA
   }
 
   const int64_t prefix_line = (int64_t)H * pl.group_at[G], line = prefix_line + (int64_t)H * pl.seq_at[B];
-  if (line == 0) return;
-  const int W = sp_workers(line, gridDim.x);
-  if (worker >= W) return;
-  int64_t at = sp_begin(worker, line, W);
-  const int64_t lo = at, hi = sp_begin(worker + 1, line, W);
-  const int slots_p = s.max_prefix_items;
+  const int64_t share = sp_share(line, gridDim.x);
+  const int64_t lo = (int64_t)worker * share;
+  if (lo >= line) return;
+  const int64_t hi = lo + share < line ? lo + share : line;
 
-  // prefix items
-  while (at < hi && at < prefix_line) {
-    const int gr = last_le(pl.group_at, G, at / H);
-    const int tiles = pl.row_tiles[gr + 1] - pl.row_tiles[gr];
-    const int steps = sp_steps(0, pl.len[gr], s.p.wt);
-    const int cost = sp_item_cost(steps, s.p.cost);
-    const int64_t g_at = (int64_t)H * pl.group_at[gr];
-    const int idx = (int)((at - g_at) / cost);  // kv head outer, row tile inner
-    const int64_t i_at = g_at + (int64_t)idx * cost;
-    const int s0 = sp_step_from(lo, i_at, steps, s.p.cost), s1 = sp_step_from(hi, i_at, steps, s.p.cost);
-    at = i_at + cost;
-    if (s1 <= s0) continue;
-    const int item = H * pl.row_tiles[gr] + idx;
-    Piece pc;
-    pc.prefix = true;
-    pc.b0 = __builtin_amdgcn_readfirstlane(pl.first[gr]);
-    pc.h = __builtin_amdgcn_readfirstlane(idx / tiles);
-    pc.row0 = __builtin_amdgcn_readfirstlane((idx % tiles) * s.p.rows);
-    pc.nrows = __builtin_amdgcn_readfirstlane((pl.first[gr + 1] - pl.first[gr]) * s.eq);
-    pc.begin = 0;
-    pc.end = __builtin_amdgcn_readfirstlane(pl.len[gr]);
-    pc.tile = __builtin_amdgcn_readfirstlane(s0 * s.p.wt);
-    pc.tile_end = __builtin_amdgcn_readfirstlane(pa_min(s1 * s.p.wt, pa_cdiv(pc.end, SP_TILE)));
-    pc.wt = s.p.wt;
-    pc.waves_r = s.p.waves_r;
-    pc.rows_out = s.p.rows;
-    const int slot = __builtin_amdgcn_readfirstlane(item + worker);
-    pc.ml = s.p_ml + (int64_t)slot * 2 * s.p.rows;
-    pc.o = s.p_o + (int64_t)slot * s.p.rows * D;
-    if (s0 == 0 && threadIdx.x == 0) {
-      const int last = sp_worker_of(i_at + SP_OVERHEAD + (int64_t)(steps - 1) * s.p.cost, line, W);
-      s.items[item] = int2{item + worker, last - worker + 1};
-    }
-    if constexpr (D <= 128) {
-      if (s.p.nr == 2)
-        run_piece<D, F16, PT, 2>(s, pc, work);
-      else
-        run_piece<D, F16, PT, 1>(s, pc, work);
+  // The item that holds position lo, then those behind it: `of` a group or a
+  // sequence, `idx` the item among its own (kv head outer, row tile inner).
+  bool prefix = lo < prefix_line;
+  int of = __builtin_amdgcn_readfirstlane(prefix ? last_le(pl.group_at, G, lo, H)
+                                                 : last_le(pl.seq_at, B, lo - prefix_line, H));
+  int idx = -1;
+  int64_t at = 0;  // of item idx
+  while (true) {
+    const SpShape& sh = prefix ? s.p : s.s;
+    int begin, end, tiles;
+    if (prefix) {
+      tiles = pl.row_tiles[of + 1] - pl.row_tiles[of];
+      begin = 0;
+      end = pl.len[of];
     } else {
-      run_piece<D, F16, PT, 1>(s, pc, work);
+      const int gr = group_of(pl, G, of);
+      tiles = s.col_tiles;
+      begin = gr >= 0 ? pl.len[gr] : 0;
+      end = context_of(s, of);
     }
-  }
-  // suffix items
-  while (at < hi) {
-    const int64_t rel = at - prefix_line;
-    const int b = last_le(pl.seq_at, B, rel / H);
-    const int gr = group_of(pl, G, b);
-    const int begin = gr >= 0 ? pl.len[gr] : 0, end = context_of(s, b);
-    const int steps = sp_steps(begin, end, s.s.wt);
-    const int cost = sp_item_cost(steps, s.s.cost);
-    const int64_t b_at = (int64_t)H * pl.seq_at[b];
-    const int idx = (int)((rel - b_at) / cost);  // kv head outer, column tile inner
-    const int64_t i_at = prefix_line + b_at + (int64_t)idx * cost;
-    const int s0 = sp_step_from(lo, i_at, steps, s.s.cost), s1 = sp_step_from(hi, i_at, steps, s.s.cost);
-    at = i_at + cost;
-    if (s1 <= s0) continue;
-    const int item = b * H * s.col_tiles + idx;
-    Piece pc;
-    pc.prefix = false;
-    pc.b0 = __builtin_amdgcn_readfirstlane(b);
-    pc.h = __builtin_amdgcn_readfirstlane(idx / s.col_tiles);
-    pc.row0 = __builtin_amdgcn_readfirstlane((idx % s.col_tiles) * s.s.rows);
-    pc.nrows = s.eq;
-    pc.begin = __builtin_amdgcn_readfirstlane(begin);
-    pc.end = __builtin_amdgcn_readfirstlane(end);
-    const int base = pc.begin / SP_TILE;
-    pc.tile = base + __builtin_amdgcn_readfirstlane(s0 * s.s.wt);
-    pc.tile_end = pa_min(base + __builtin_amdgcn_readfirstlane(s1 * s.s.wt), pa_cdiv(pc.end, SP_TILE));
-    pc.wt = s.s.wt;
-    pc.waves_r = s.s.waves_r;
-    pc.rows_out = s.s_rows;
-    const int slot = __builtin_amdgcn_readfirstlane(item + worker);
-    pc.ml = s.s_ml + (int64_t)slot * 2 * s.s_rows;
-    pc.o = s.s_o + (int64_t)slot * s.s_rows * D;
-    if (s0 == 0 && threadIdx.x == 0) {
-      const int last = sp_worker_of(i_at + SP_OVERHEAD + (int64_t)(steps - 1) * s.s.cost, line, W);
-      s.items[slots_p + item] = int2{item + worker, last - worker + 1};
+    tiles = __builtin_amdgcn_readfirstlane(tiles);
+    begin = __builtin_amdgcn_readfirstlane(begin);
+    end = __builtin_amdgcn_readfirstlane(end);
+    const int steps = sp_steps(begin, end, sh.tiles);
+    const int cost = sp_item_cost(steps, sh.cost);
+    const int64_t of_at = prefix ? (int64_t)H * pl.group_at[of] : prefix_line + (int64_t)H * pl.seq_at[of];
+    if (idx < 0) {  // the first one
+      idx = sp_worker_of(lo - of_at, cost);
+      at = of_at + (int64_t)idx * cost;
     }
-    if constexpr (D <= 128) {
-      if (s.s.nr == 2)
-        run_piece<D, F16, PT, 2>(s, pc, work);
-      else
-        run_piece<D, F16, PT, 1>(s, pc, work);
-    } else {
-      run_piece<D, F16, PT, 1>(s, pc, work);
+    for (; idx < H * tiles && at < hi; ++idx, at += cost) {
+      const int s0 = sp_step_from(lo, at, steps, sh.cost), s1 = sp_step_from(hi, at, steps, sh.cost);
+      if (s1 <= s0) continue;
+      const int item = prefix ? H * pl.row_tiles[of] + idx : of * H * tiles + idx;
+      const int t0 = begin / SP_TILE, h = idx / tiles;
+      const int slot = __builtin_amdgcn_readfirstlane(item + worker);
+      Piece pc;
+      pc.b0 = prefix ? __builtin_amdgcn_readfirstlane(pl.first[of]) : of;
+      pc.h = __builtin_amdgcn_readfirstlane(h);
+      pc.row0 = __builtin_amdgcn_readfirstlane((idx - h * tiles) * sh.rows);
+      pc.nrows = prefix ? __builtin_amdgcn_readfirstlane((pl.first[of + 1] - pl.first[of]) * s.eq) : s.eq;
+      pc.begin = begin;
+      pc.end = end;
+      pc.tile = __builtin_amdgcn_readfirstlane(t0 + s0 * sh.tiles);
+      pc.tile_end = __builtin_amdgcn_readfirstlane(pa_min(t0 + s1 * sh.tiles, pa_cdiv(end, SP_TILE)));
+      pc.rows_out = prefix ? s.p.rows : s.s_rows;
+      pc.ml = (prefix ? s.p_ml : s.s_ml) + (int64_t)slot * 2 * pc.rows_out;
+      pc.o = (prefix ? s.p_o : s.s_o) + (int64_t)slot * pc.rows_out * D;
+      if (s0 == 0 && threadIdx.x == 0) {
+        const int last = sp_worker_of(at + SP_OVERHEAD + (int64_t)(steps - 1) * sh.cost, share);
+        s.items[prefix ? item : s.max_prefix_items + item] = int2{item + worker, last - worker + 1};
+      }
+      run_piece<D, F16, PT>(s, sh, pc, work);
     }
+    if (at >= hi) return;
+    // on to the next group or sequence that has items
+    idx = 0;
+    ++of;
+    if (prefix) {
+      while (of < G && pl.group_at[of + 1] == pl.group_at[of]) ++of;
+      if (of >= G) {
+        prefix = false;
+        of = 0;
+      }
+    }
+    if (!prefix)
+      while (of < B && pl.seq_at[of + 1] == pl.seq_at[of]) ++of;
+    if (!prefix && of >= B) return;
+    of = __builtin_amdgcn_readfirstlane(of);
   }
 }
 
@@ -785,7 +958,7 @@ int sizes_of(int B, int G, int H, int ql, int gqa, int D, int workers, Sizes* z)
 
 template <int D, bool F16, bool PT>
 hipError_t launch(const SpArgs& s, hipStream_t st) {
-  const int lds = plan_bytes(s.a.num_seqs, s.a.num_groups) + end_bytes(pa_max(s.p.nr, s.s.nr));
+  const int lds = plan_bytes(s.a.num_seqs, s.a.num_groups) + work_bytes(D, (s.a.num_groups > 0 && s.p.shared) || s.s.shared);
   hipLaunchKernelGGL((pa_shared_prefix_kernel<D, F16, PT>), dim3(s.a.num_workers), dim3(kThreads), lds, st, s);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
@@ -842,32 +1015,32 @@ extern "C" int pa_fp8_plan_shared_prefix(const int32_t* context_lengths, const i
     len[g] = rows > 0 ? pa_min(pa_max(prefix_lengths[g], 0), capacity) : 0;
     for (int b = first[g]; b < first[g + 1]; ++b) seq_len[b] = len[g];
     tiles[g + 1] = tiles[g] + (len[g] > 0 ? pa_cdiv(rows, z.p.rows) : 0);
-    const int n = tiles[g + 1] - tiles[g], steps = sp_steps(0, len[g], z.p.wt);
+    const int n = tiles[g + 1] - tiles[g], steps = sp_steps(0, len[g], z.p.tiles);
     if (n > 0) line.push_back({true, g, n, H * n, 0, steps, len[g], H * tiles[g]});
     total += (int64_t)H * n * sp_item_cost(steps, z.p.cost);
   }
   for (int b = 0; b < B; ++b) {
     const int end = pa_min(pa_max(context_lengths[b], 0), capacity);
-    const int steps = sp_steps(seq_len[b], end, z.s.wt);
+    const int steps = sp_steps(seq_len[b], end, z.s.tiles);
     if (steps > 0) line.push_back({false, b, z.col_tiles, H * z.col_tiles, seq_len[b], steps, end, b * H * z.col_tiles});
     total += (int64_t)H * z.col_tiles * sp_item_cost(steps, z.s.cost);
   }
   if (total == 0) return 0;
-  const int W = sp_workers(total, workers);
+  const int64_t share = sp_share(total, workers);
   int n = 0;
   int64_t at = 0;
   for (const Kind& k : line) {
     const SpShape& sh = k.prefix ? z.p : z.s;
     for (int i = 0; i < k.items; ++i) {
-      const int w0 = sp_worker_of(at + SP_OVERHEAD, total, W);
-      const int w1 = sp_worker_of(at + SP_OVERHEAD + (int64_t)(k.steps - 1) * sh.cost, total, W);
+      const int w0 = sp_worker_of(at + SP_OVERHEAD, share);
+      const int w1 = sp_worker_of(at + SP_OVERHEAD + (int64_t)(k.steps - 1) * sh.cost, share);
       for (int w = w0; w <= w1; ++w) {
-        const int s0 = sp_step_from(sp_begin(w, total, W), at, k.steps, sh.cost);
-        const int s1 = sp_step_from(sp_begin(w + 1, total, W), at, k.steps, sh.cost);
+        const int s0 = sp_step_from(w * share, at, k.steps, sh.cost);
+        const int s1 = sp_step_from((w + 1) * share, at, k.steps, sh.cost);
         if (n < max_pieces) {
           const int t0 = k.begin / SP_TILE;
-          const int32_t rec[8] = {k.prefix, k.base + i, w, k.base + i + w, k.of, i / k.h0, t0 + s0 * sh.wt,
-                                  pa_min(t0 + s1 * sh.wt, pa_cdiv(k.end, SP_TILE))};
+          const int32_t rec[8] = {k.prefix, k.base + i, w, k.base + i + w, k.of, i / k.h0, t0 + s0 * sh.tiles,
+                                  pa_min(t0 + s1 * sh.tiles, pa_cdiv(k.end, SP_TILE))};
           for (int j = 0; j < 8; ++j) pieces[8 * n + j] = rec[j];
         }
         ++n;

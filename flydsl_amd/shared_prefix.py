@@ -39,6 +39,11 @@ MAX_SEQS = 4096
 MAX_GROUPS = 1024
 
 
+def _workers(device) -> int:
+    """Persistent workgroups of a launch: two fit a compute unit."""
+    return 2 * _cu_count(device)
+
+
 class PreparedSharedPrefix:
     """A validated call with its C-ABI arguments marshalled; ``launch()``
     issues it.  The tensors must stay alive and unchanged in shape; launches
@@ -104,7 +109,7 @@ def pa_decode_shared_prefix(
     native = _lib.native()
     if native is not None and stream is None and native.shared_prefix(
             output, query, key_cache, value_cache, context_lengths, block_tables, prefix_indptr, prefix_lengths,
-            softmax_scale, key_scale, value_scale, _cu_count):
+            softmax_scale, key_scale, value_scale, _workers):
         return ROUTE
     return prepare_pa_decode_shared_prefix(
         output, query, key_cache, value_cache, context_lengths, block_tables, prefix_indptr, prefix_lengths,
@@ -222,7 +227,7 @@ def prepare_pa_decode_shared_prefix(
     a.per_token_kv, a.trans_v = int(per_token), int(trans_v)
     a.query_dtype = DTYPE_BF16 if dtype == "bf16" else DTYPE_F16
     a.output_dtype = out_dtype
-    a.num_workers = _cu_count(dev)
+    a.num_workers = _workers(dev)
     a.softmax_scale = float(softmax_scale)
     keep = (output, query, key_cache, value_cache, context_lengths, block_tables, prefix_indptr, prefix_lengths,
             key_scale, value_scale)

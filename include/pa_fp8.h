@@ -631,7 +631,7 @@ int pa_fp8_fnuz_to_fn(const void* src, const int32_t* rows, int64_t num_rows, in
  * Head sizes 64, 128, 192 and 256; page sizes 16, 32, ..., 1024 (powers of
  * two); at most 4096 sequences and 1024 groups.  Two launches; the workspace
  * (pa_fp8_shared_prefix_workspace_bytes) needs no initialisation and is the
- * call's own until the launches end.  num_workers: persistent workgroups, one
+ * call's own until the launches end.  num_workers: persistent workgroups, two
  * per compute unit.  16-byte alignment: query strides are multiples of 8
  * elements, cache strides of 16 bytes, output and per-token scale strides of 4
  * elements.

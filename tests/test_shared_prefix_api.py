@@ -58,7 +58,7 @@ def test_marshalling():
                          per_token=True, extra_cols=2)
     a = prep(c).args
     assert (a.num_seqs, a.num_groups, a.num_kv_heads, a.query_length, a.query_group_size) == (4, 1, 2, 1, 4)
-    assert (a.head_size, a.block_size, a.per_token_kv, a.trans_v, a.num_workers) == (128, 32, 1, 1, 256)
+    assert (a.head_size, a.block_size, a.per_token_kv, a.trans_v, a.num_workers) == (128, 32, 1, 1, 512)
     assert a.num_blocks == c["key_cache"].shape[0] and a.max_blocks_per_seq == c["block_tables"].shape[1]
     assert a.stride_bt_seq == c["block_tables"].stride(0) and a.stride_ks_block == 64 and a.stride_ks_head == 32
     assert a.prefix_indptr == c["prefix_indptr"].data_ptr() and a.prefix_lengths == c["prefix_lengths"].data_ptr()

@@ -14,11 +14,11 @@ TILE = 64
 
 
 def rows_of(eq, d):
-    nr = 2 if eq > 16 and d <= 128 else 1
-    w = 1
-    while w < 8 and 16 * nr * w < eq:
-        w *= 2
-    return 16 * nr * w, 8 // w
+    """Rows of an item."""
+    most = 2 if d <= 128 else 1
+    if eq <= 16 and d <= 128:
+        return 16
+    return 32 if eq <= 32 else 64 if eq <= 64 else 64 * most
 
 
 def check(ctx, indptr, prefix, hkv, ql, gqa, d, capacity, workers):
@@ -27,8 +27,7 @@ def check(ctx, indptr, prefix, hkv, ql, gqa, d, capacity, workers):
     first = np.maximum.accumulate(np.clip(indptr, 0, B)) if G else np.zeros(1, int)
     own = [0] * B
     want = {}  # (prefix, item) -> (of, head, first tile, end tile)
-    p_rows, _ = rows_of(-(-B * eq // max(G, 1)), d)
-    s_rows, _ = rows_of(eq, d)
+    p_rows, s_rows = rows_of(-(-B * eq // max(G, 1)), d), rows_of(eq, d)
     item = 0
     for g in range(G):
         rows = (first[g + 1] - first[g]) * eq
@@ -111,8 +110,7 @@ def test_shares_are_even():
     pieces = check([17000 + i for i in range(256)], [0, 256], [16383], 8, 1, 4, 128, 1 << 20, 256)
     cost = np.zeros(256)
     for is_p, _, w, _, _, _, t0, t1 in pieces.tolist():
-        wt, c = (1, 8) if is_p else (8, 5)
-        cost[w] += 6 + -(-(t1 - t0) // wt) * c
+        cost[w] += 6 + ((t1 - t0) * 4 if is_p else -(-(t1 - t0) // 4) * 8)
     assert cost.max() <= cost.mean() + 8 + 12
 
 
