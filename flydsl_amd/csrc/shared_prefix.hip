@@ -146,58 +146,69 @@ __device__ __forceinline__ uint32_t keep4(int t, int lo, int hi) {
 struct Plan {
   int64_t* seq_at;    // [B + 1] cost of the sequences' items before b, one kv head
   int64_t* group_at;  // [G + 1] likewise of the groups' prefix items
-  int* first;         // [G + 1] first sequence of a group (never falls)
-  int* len;           // [G] prefix length
-  int* row_tiles;     // [G + 1] prefix items of the groups before g, one kv head
   int64_t* scratch;   // [SP_WAVES]
+  int* ctx;           // [B] context length, at most what a table row holds
+  int* first;         // [G + 1] first sequence of a group (never falls)
+  int* len;           // [G + 1] prefix length
+  int* row_tiles;     // [G + 1] prefix items of the groups before g, one kv head
 };
 
 __host__ __device__ inline int plan_bytes(int B, int G) {
-  return (8 * (B + 1) + 8 * (G + 1) + 8 * SP_WAVES + 4 * (G + 1) + 4 * (G + 1) + 4 * (G + 1) + 15) & ~15;
+  return (8 * (B + 1) + 8 * (G + 1) + 8 * SP_WAVES + 4 * B + 12 * (G + 1) + 15) & ~15;
 }
 __device__ __forceinline__ Plan plan_of(char* lds, int B, int G) {
   Plan p;
   p.seq_at = (int64_t*)lds;
   p.group_at = p.seq_at + B + 1;
   p.scratch = p.group_at + G + 1;
-  p.first = (int*)(p.scratch + SP_WAVES);
+  p.ctx = (int*)(p.scratch + SP_WAVES);
+  p.first = p.ctx + B;
   p.len = p.first + G + 1;
   p.row_tiles = p.len + G + 1;
   return p;
 }
 
-// a[0 .. n] := the sums (MAX: maxima, inclusive) of what stands before each
-// entry; every thread of the workgroup calls it, between barriers of its own.
+// Inclusive sums (MAX: maxima) over the wave.
+template <bool MAX, typename T>
+__device__ __forceinline__ T wave_upto(T v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const T o = sizeof(T) == 8 ? (T)__shfl_up((long long)v, d, 64) : (T)__shfl_up((int)v, d, 64);
+    if (lane >= d) v = MAX ? (o > v ? o : v) : v + o;
+  }
+  return v;
+}
+
+// a[0 .. n] := the sums (MAX: a[0 .. n - 1] := the maxima, inclusive) of what
+// stands before each entry; the workgroup calls it with a[] written and visible.
 template <bool MAX, typename T>
 __device__ void block_scan(T* a, int n, int64_t* scratch) {
   const int per = (n + kThreads - 1) / kThreads;
   const int i0 = threadIdx.x * per, i1 = pa_min(i0 + per, n);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  auto op = [](int64_t x, int64_t y) { return MAX ? (x > y ? x : y) : x + y; };
-  __syncthreads();
-  int64_t mine = 0;
-  for (int i = i0; i < i1; ++i) mine = op(mine, (int64_t)a[i]);
-  int64_t upto = mine;
-  for (int d = 1; d < 64; d *= 2) {
-    const int64_t o = __shfl_up((long long)upto, d, 64);
-    if (lane >= d) upto = op(upto, o);
-  }
-  if (lane == 63) scratch[wave] = upto;
-  int64_t before = __shfl_up((long long)upto, 1, 64);
+  T mine = 0;
+  for (int i = i0; i < i1; ++i) mine = MAX ? (a[i] > mine ? a[i] : mine) : mine + a[i];
+  const T upto = wave_upto<MAX>(mine);
+  if (lane == 63) scratch[wave] = (int64_t)upto;
+  T before = sizeof(T) == 8 ? (T)__shfl_up((long long)upto, 1, 64) : (T)__shfl_up((int)upto, 1, 64);
   if (lane == 0) before = 0;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) before = op(before, scratch[w]);
+  for (int w = 0; w < wave; ++w) {
+    const T o = (T)scratch[w];
+    before = MAX ? (o > before ? o : before) : before + o;
+  }
   for (int i = i0; i < i1; ++i) {
-    const int64_t v = (int64_t)a[i];
+    const T v = a[i];
     if (MAX) {
-      before = op(before, v);
-      a[i] = (T)before;
+      before = v > before ? v : before;
+      a[i] = before;
     } else {
-      a[i] = (T)before;
+      a[i] = before;
       before += v;
     }
   }
-  if (!MAX && i0 < n && i1 == n) a[n] = (T)before;
+  if (!MAX && i0 < n && i1 == n) a[n] = before;
   if (!MAX && n == 0 && threadIdx.x == 0) a[0] = 0;
   __syncthreads();
 }
@@ -222,33 +233,67 @@ __device__ __forceinline__ int group_of(const Plan& p, int G, int b) {
   return last_le(p.first, G, b);
 }
 
-__device__ __forceinline__ int context_of(const SpArgs& s, int b) {
-  const int n = s.a.context_lengths[b];
-  return n < 0 ? 0 : (n < s.capacity ? n : s.capacity);
+// Prefix length, prefix items and their cost of group g, whose first[] is set.
+__device__ __forceinline__ void plan_group(const SpArgs& s, int sequences, int given, int* len, int* tiles, int64_t* cost) {
+  const int rows = sequences * s.eq;
+  *len = rows > 0 ? pa_min(pa_max(given, 0), s.capacity) : 0;
+  *tiles = *len > 0 ? pa_cdiv(rows, s.p.rows) : 0;
+  *cost = (int64_t)*tiles * sp_item_cost(sp_steps(0, *len, s.p.tiles), s.p.cost);
 }
 
+// Every workgroup makes the whole plan: two rounds of loads (all lengths, then
+// none) and a few barriers, 1 us, where a launch of its own would take 3.
 __device__ void make_plan(const Plan& p, const SpArgs& s) {
   const int B = s.a.num_seqs, G = s.a.num_groups;
-  if (G > 0) {
-    for (int g = threadIdx.x; g <= G; g += kThreads) p.first[g] = pa_min(pa_max(s.a.prefix_indptr[g], 0), B);
+  for (int b = threadIdx.x; b < B; b += kThreads) {
+    const int n = s.a.context_lengths[b];
+    p.ctx[b] = n < 0 ? 0 : (n < s.capacity ? n : s.capacity);
+  }
+  if (G < 64) {  // the groups in one wave's lanes
+    if (threadIdx.x < 64) {
+      const int g = threadIdx.x;
+      int f = 0, given = 0;
+      if (G > 0 && g <= G) f = pa_min(pa_max(s.a.prefix_indptr[g], 0), B);
+      if (g < G) given = s.a.prefix_lengths[g];
+      f = wave_upto<true>(f);
+      const int next = __shfl_down(f, 1, 64);
+      int len = 0, tiles = 0;
+      int64_t cost = 0;
+      if (g < G) plan_group(s, next - f, given, &len, &tiles, &cost);
+      const int tiles_upto = wave_upto<false>(tiles);
+      const int64_t cost_upto = wave_upto<false>(cost);
+      if (g <= G) {
+        p.first[g] = f;
+        p.len[g] = len;
+        p.row_tiles[g] = tiles_upto - tiles;
+        p.group_at[g] = cost_upto - cost;
+      }
+    }
+    __syncthreads();
+  } else {
+    for (int g = threadIdx.x; g <= G; g += kThreads) {
+      p.first[g] = pa_min(pa_max(s.a.prefix_indptr[g], 0), B);
+      p.len[g] = g < G ? s.a.prefix_lengths[g] : 0;
+    }
+    __syncthreads();
     block_scan<true>(p.first, G + 1, p.scratch);
     for (int g = threadIdx.x; g < G; g += kThreads) {
-      const int rows = (p.first[g + 1] - p.first[g]) * s.eq;
-      const int len = rows > 0 ? pa_min(pa_max(s.a.prefix_lengths[g], 0), s.capacity) : 0;
-      const int tiles = len > 0 ? pa_cdiv(rows, s.p.rows) : 0;
+      int len, tiles;
+      int64_t cost;
+      plan_group(s, p.first[g + 1] - p.first[g], p.len[g], &len, &tiles, &cost);
       p.len[g] = len;
       p.row_tiles[g] = tiles;
-      p.group_at[g] = (int64_t)tiles * sp_item_cost(sp_steps(0, len, s.p.tiles), s.p.cost);
+      p.group_at[g] = cost;
     }
+    __syncthreads();
     block_scan<false>(p.row_tiles, G, p.scratch);
     block_scan<false>(p.group_at, G, p.scratch);
-  } else if (threadIdx.x == 0) {
-    p.group_at[0] = 0;
   }
-  for (int b = threadIdx.x; b < B; b += kThreads) {
+  const int per = (B + kThreads - 1) / kThreads;  // (block_scan's own split: no barrier between)
+  for (int b = threadIdx.x * per; b < pa_min((int)(threadIdx.x + 1) * per, B); ++b) {
     const int g = group_of(p, G, b);
     const int len = g >= 0 ? p.len[g] : 0;
-    p.seq_at[b] = (int64_t)s.col_tiles * sp_item_cost(sp_steps(len, context_of(s, b), s.s.tiles), s.s.cost);
+    p.seq_at[b] = (int64_t)s.col_tiles * sp_item_cost(sp_steps(len, p.ctx[b], s.s.tiles), s.s.cost);
   }
   block_scan<false>(p.seq_at, B, p.scratch);
 }
@@ -268,16 +313,11 @@ struct Piece {
   float* o;
 };
 
-// LDS behind the plan: two buffers of a tile's keys and values in 16 bits and
-// their scales, or, at a piece's end, maxima and sums by wave and 32 output
-// dims of every row.
+// LDS behind the plan: two buffers of a tile (run_shared), or, at a piece's end,
+// maxima and sums by wave and 32 output dims of every row.
 constexpr int kOutStride = 36;  // floats a row of 32 dims takes (16-byte steps that spread over the banks)
 __host__ __device__ constexpr int end_bytes(int nr) {
   return SP_WAVES * 16 * nr * 4 * 2 + SP_WAVES * 16 * nr * kOutStride * 4;
-}
-__host__ __device__ constexpr int tile_bytes(int d) { return 2 * SP_TILE * d * 2; }
-__host__ __device__ constexpr int work_bytes(int d, bool shared) {
-  return shared ? 2 * (tile_bytes(d) + 2 * SP_TILE * 4) : end_bytes(d <= 128 ? 2 : 1);
 }
 
 // The wave's rows: operand B of the key product, the keys each row sees, and
@@ -331,39 +371,51 @@ struct Rows {
   }
 
   // Softmax of NT tiles' logits x (tokens t0 + 16 g + 4 (T0 + T) + i of the lane's
-  // row n) against the row's reference; p: the probabilities (times vs) as
-  // operands.
+  // row of each n) against the rows' references; p: the probabilities (times
+  // vs) as operands.
   template <bool PT, bool PF16, int NT>
-  __device__ __forceinline__ void softmax(int n, const f32x4 (&x)[NT], const f32x4 (&vs)[NT], i32x4 (&p)[NT / 2]) {
-    float top = kNegInf;
+  __device__ __forceinline__ void softmax(const f32x4 (&x)[NR][NT], const f32x4 (&vs)[NT], i32x4 (&p)[NR][NT / 2]) {
+    float top[NR];
+    bool moves = false;
 #pragma unroll
-    for (int T = 0; T < NT; ++T)
+    for (int n = 0; n < NR; ++n) {
+      top[n] = kNegInf;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) top = fmaxf(top, x[T][i]);
-    top = groups_max(top) * fac;
-    if (__ballot(top > m[n] + kRescaleMargin)) {
-      const float mn = fmaxf(m[n], top);
-      const float f = mn == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m[n] - mn);
-      l[n] *= f;
+      for (int T = 0; T < NT; ++T)
 #pragma unroll
-      for (int dt = 0; dt < D / 16; ++dt) o[n][dt] *= f;
-      m[n] = mn;
+        for (int i = 0; i < 4; ++i) top[n] = fmaxf(top[n], x[n][T][i]);
+      top[n] = groups_max(top[n]) * fac;
+      moves |= top[n] > m[n] + kRescaleMargin;
     }
-    const float bias = m[n] == kNegInf ? 0.0f : -m[n];
-    float w[4 * NT], sum = 0.0f;
+    if (__ballot(moves)) {
 #pragma unroll
-    for (int T = 0; T < NT; ++T)
+      for (int n = 0; n < NR; ++n) {
+        const float mn = top[n] > m[n] + kRescaleMargin ? top[n] : m[n];
+        const float f = mn == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m[n] - mn);
+        l[n] *= f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[T][i], fac, bias));
-        sum += e;
-        w[4 * T + i] = PT ? e * vs[T][i] : e;
+        for (int dt = 0; dt < D / 16; ++dt) o[n][dt] *= f;
+        m[n] = mn;
       }
-    l[n] += sum;
+    }
 #pragma unroll
-    for (int j = 0; j < NT / 2; ++j)
+    for (int n = 0; n < NR; ++n) {
+      const float bias = m[n] == kNegInf ? 0.0f : -m[n];
+      float w[4 * NT], sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[j][i] = round2<PF16>(w[8 * j + 2 * i], w[8 * j + 2 * i + 1]);
+      for (int T = 0; T < NT; ++T)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][T][i], fac, bias));
+          sum += e;
+          w[4 * T + i] = PT ? e * vs[T][i] : e;
+        }
+      l[n] += sum;
+#pragma unroll
+      for (int j = 0; j < NT / 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[n][j][i] = round2<PF16>(w[8 * j + 2 * i], w[8 * j + 2 * i + 1]);
+    }
   }
 
   // Joins the waves of the same rows (wt of them, this one the wi-th) and writes
@@ -441,6 +493,18 @@ struct Pages {
   }
 };
 
+// The same for a token all lanes ask for: a scalar load (the launch writes no table).
+struct ScalarPages : Pages {
+  __device__ __forceinline__ ScalarPages(const SpArgs& s, const Piece& pc) : Pages(s, pc) {}
+  __device__ __forceinline__ int operator()(int token) const {
+    const int i = __builtin_amdgcn_readfirstlane(pa_min(token >> lbs, last));
+    int p = ((const __attribute__((address_space(4))) int32_t*)table)[i];
+    pa_note(p < 0 || p >= blocks, PA_VIOLATION_PAGE);
+    p = p < 0 ? 0 : p;
+    return p < blocks ? p : blocks - 1;
+  }
+};
+
 template <int D, bool F16, bool PT>
 __device__ __forceinline__ void run_direct(const SpArgs& s, const Piece& pc, char* lds) {
   // the value product of f16 queries with per-token scales runs in bf16: a
@@ -500,32 +564,33 @@ __device__ __forceinline__ void run_direct(const SpArgs& s, const Piece& pc, cha
   for (; tile < pc.tile_end; tile += SP_WAVES) {
     const int next = tile + SP_WAVES;
     const bool more = next < pc.tile_end;
-    f32x4 x[4];
+    f32x4 x[1][4];
 #pragma unroll
     for (int T = 0; T < 4; ++T) {
-      x[T] = f32x4{0.f, 0.f, 0.f, 0.f};
+      x[0][T] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int u = 0; u < D / 64; ++u) {
         const i32x4 k0 = widen8<F16>(kr[T][u][0], kr[T][u][1]), k1 = widen8<F16>(kr[T][u][2], kr[T][u][3]);
-        x[T] = mfma<F16>(k0, w.q[0][2 * u], x[T]);
-        x[T] = mfma<F16>(k1, w.q[0][2 * u + 1], x[T]);
+        x[0][T] = mfma<F16>(k0, w.q[0][2 * u], x[0][T]);
+        x[0][T] = mfma<F16>(k1, w.q[0][2 * u + 1], x[0][T]);
       }
     }
     if (more) load_keys(next, kp);
     if constexpr (PT) {
 #pragma unroll
-      for (int T = 0; T < 4; ++T) x[T] *= ks[T];
+      for (int T = 0; T < 4; ++T) x[0][T] *= ks[T];
       if (more) load_scales(a.key_scale, next, vp, ks);
     }
     // ---- masks: the part's first and last tiles ----
     const int t0 = tile * SP_TILE;
     if (t0 < pc.begin || t0 + SP_TILE > pa_min(w.least, pc.end)) {
+      asm volatile("");  // (a branch: not computed for every tile)
 #pragma unroll
       for (int T = 0; T < 4; ++T)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int t = t0 + 16 * g + 4 * T + i;
-          if (t < pc.begin || t >= w.limit[0]) x[T][i] = kNegInf;
+          if (t < pc.begin || t >= w.limit[0]) x[0][T][i] = kNegInf;
         }
       // bytes behind the part's tokens may be anything, NaN among it
 #pragma unroll
@@ -544,13 +609,13 @@ __device__ __forceinline__ void run_direct(const SpArgs& s, const Piece& pc, cha
           }
       }
     }
-    i32x4 p[2];
-    w.template softmax<PT, PF16, 4>(0, x, vs, p);
+    i32x4 p[1][2];
+    w.template softmax<PT, PF16, 4>(x, vs, p);
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) {
       const i32x4 v0 = widen8<PF16>(vr[dt][0], vr[dt][1]), v1 = widen8<PF16>(vr[dt][2], vr[dt][3]);
-      w.o[0][dt] = mfma<PF16>(v0, p[0], w.o[0][dt]);
-      w.o[0][dt] = mfma<PF16>(v1, p[1], w.o[0][dt]);
+      w.o[0][dt] = mfma<PF16>(v0, p[0][0], w.o[0][dt]);
+      w.o[0][dt] = mfma<PF16>(v1, p[0][1], w.o[0][dt]);
     }
     if (more) {
       load_values(next, vp);
@@ -564,8 +629,19 @@ __device__ __forceinline__ void run_direct(const SpArgs& s, const Piece& pc, cha
 }
 
 // A tile in LDS, 16-byte pieces: keys [D / 8 octets of dims][64 rows of the key
-// tiles], values [8 octets of tokens][D dims] -- an operand read takes 16
-// consecutive pieces a lane group, and so does a wave's write.
+// tiles], values [8 octets of tokens][D dims].  An operand read takes 16
+// consecutive pieces a lane group; the key tiles of an octet stand 320 bytes
+// apart, so that a wave's writes of a block's tokens (four of each key tile)
+// meet different banks.
+constexpr int kKeyTile = 320 / 16, kKeyRow = 4 * kKeyTile;  // pieces
+__host__ __device__ constexpr int tile_bytes(int d) {
+  return d / 8 * kKeyRow * 16 + SP_TILE * d * 2 + 2 * SP_TILE * 4;
+}
+
+__host__ __device__ constexpr int work_bytes(int d, bool shared) {
+  return shared ? 2 * tile_bytes(d) : end_bytes(1);
+}
+
 template <int D, bool F16, bool PT, int NR, int WT>
 __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, char* lds) {
   constexpr bool PF16 = F16 && !PT;
@@ -576,98 +652,93 @@ __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, cha
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wave / WT, wi = wave % WT;
   const int bs = 1 << s.lbs;
-  const Pages page_of(s, pc);
+
+  // Wave w brings token block w of each tile: one page, so its addresses are
+  // scalar but for a lane's constant offset.  Of the keys, lane (c, g) has token c
+  // and dims 16 (g + 4 i) .. + 15; of the values, dims lane + 64 i; of the scales,
+  // token c of the keys' (g = 0) or the values' (g = 1).
+  const ScalarPages page_of(s, pc);
   const uint8_t* kbase = (const uint8_t*)a.key_cache + (int64_t)pc.h * a.stride_k_head;
   const uint8_t* vbase = (const uint8_t*)a.value_cache + (int64_t)pc.h * a.stride_v_head;
+  const int64_t s_head = (int64_t)pc.h * a.stride_ks_head;
   const int v_dim = a.trans_v ? 16 : bs, v_blk = a.trans_v ? D * 16 : 16;
-  const float* ks_base = (threadIdx.x < SP_TILE ? a.key_scale : a.value_scale) + (int64_t)pc.h * a.stride_ks_head;
-
-  // what this thread brings: row `lane` of the key tiles, dims 16 (wave + 4 i); of
-  // piece threadIdx.x + 256 i of the values, its dim and token block
-  const int k_tok = 16 * ((lane & 15) >> 2) + 4 * (lane >> 4) + (lane & 3);
+  const uint32_t k_lane = (uint32_t)(c * 16 + g * (bs * 16)), v_lane = (uint32_t)(lane * v_dim);
+  const uint32_t k_step = (uint32_t)(bs * 64), v_step = (uint32_t)(64 * v_dim);
   i32x4 kst[NS], vst[NS];
   float sst = 0.0f;
-  int kpage, vpage[NS], spage = 0;
-  auto v_block = [&](int i) { return (int)(threadIdx.x + kThreads * i) / D; };
-  auto v_dim_of = [&](int i) { return (int)(threadIdx.x + kThreads * i) % D; };
-  auto pages = [&](int tile) {
-    kpage = page_of(tile * SP_TILE + (k_tok & ~15));
-#pragma unroll
-    for (int i = 0; i < NS; ++i) vpage[i] = page_of(tile * SP_TILE + 16 * v_block(i));
-    if constexpr (PT) spage = page_of(tile * SP_TILE + (int)(threadIdx.x & (SP_TILE - 1)));
-  };
+  int page = 0;
+  auto next_page = [&](int tile) { page = page_of(tile * SP_TILE + 16 * wave); };
   auto fetch = [&](int tile) {
-    const uint8_t* kp = kbase + (int64_t)kpage * a.stride_k_block + ((tile * SP_TILE + k_tok) & (bs - 1)) * 16;
+    const int in = (tile * SP_TILE + 16 * wave) & (bs - 1);
+    const uint8_t* kp = kbase + (int64_t)page * a.stride_k_block + in * 16;
+    const uint8_t* vp = vbase + (int64_t)page * a.stride_v_block + (in >> 4) * v_blk;
 #pragma unroll
-    for (int i = 0; i < NS; ++i) kst[i] = *(const i32x4*)(kp + (int64_t)(wave + SP_WAVES * i) * (bs * 16));
+    for (int i = 0; i < NS; ++i) kst[i] = *(const i32x4*)(kp + (k_lane + i * k_step));
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      const int in = ((tile * SP_TILE + 16 * v_block(i)) & (bs - 1)) >> 4;
-      vst[i] = *(const i32x4*)(vbase + (int64_t)vpage[i] * a.stride_v_block + in * v_blk + (int64_t)v_dim_of(i) * v_dim);
-    }
+    for (int i = 0; i < NS; ++i) vst[i] = *(const i32x4*)(vp + (v_lane + i * v_step));
     if constexpr (PT) {
-      if (threadIdx.x < 2 * SP_TILE)
-        sst = ks_base[(int64_t)spage * a.stride_ks_block + ((tile * SP_TILE + (int)(threadIdx.x & (SP_TILE - 1))) & (bs - 1))];
+      const int64_t at = (int64_t)page * a.stride_ks_block + s_head + in;
+      if (g < 2) sst = (g ? a.value_scale : a.key_scale)[at + c];
     }
   };
-  constexpr int kBuffer = tile_bytes(D) + 2 * SP_TILE * 4;
   auto store = [&](int tile, int buffer) {
-    i32x4* lk = (i32x4*)(lds + buffer * kBuffer);
-    i32x4* lv = lk + SP_TILE * D / 8;
+    i32x4* lk = (i32x4*)(lds + buffer * tile_bytes(D));
+    i32x4* lv = lk + D / 8 * kKeyRow;
     const int t0 = tile * SP_TILE;
     if (t0 < pc.begin || t0 + SP_TILE > pc.end) {  // bytes outside the part may be anything, NaN among it
+      asm volatile("");
 #pragma unroll
-      for (int i = 0; i < NS; ++i)
+      for (int k = 0; k < 4; ++k) {
+        const int keep = (int)keep4(t0 + 16 * wave + 4 * k, pc.begin, pc.end);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) vst[i][k] &= (int)keep4(t0 + 16 * v_block(i) + 4 * k, pc.begin, pc.end);
+        for (int i = 0; i < NS; ++i) vst[i][k] &= keep;
+      }
       if constexpr (PT) {
-        const int t = t0 + (int)(threadIdx.x & (SP_TILE - 1));
+        const int t = t0 + 16 * wave + c;
         if (t < pc.begin || t >= pc.end) sst = 0.0f;
       }
     }
+    const int row = (c >> 2) * kKeyTile + 4 * wave + (c & 3);  // row 4 wave + c % 4 of key tile c / 4
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
-      const int o8 = 2 * (wave + SP_WAVES * i);
-      lk[o8 * SP_TILE + lane] = widen8<F16>(kst[i][0], kst[i][1]);
-      lk[(o8 + 1) * SP_TILE + lane] = widen8<F16>(kst[i][2], kst[i][3]);
+      const int o8 = 2 * (g + 4 * i);
+      lk[o8 * kKeyRow + row] = widen8<F16>(kst[i][0], kst[i][1]);
+      lk[(o8 + 1) * kKeyRow + row] = widen8<F16>(kst[i][2], kst[i][3]);
     }
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
-      const int at = 2 * v_block(i) * D + v_dim_of(i);
+      const int at = 2 * wave * D + lane + 64 * i;
       lv[at] = widen8<PF16>(vst[i][0], vst[i][1]);
       lv[at + D] = widen8<PF16>(vst[i][2], vst[i][3]);
     }
     if constexpr (PT) {
-      if (threadIdx.x < 2 * SP_TILE) ((float*)(lv + SP_TILE * D / 8))[threadIdx.x] = sst;
+      if (g < 2) ((float*)(lv + SP_TILE * D / 8))[g * SP_TILE + 16 * wave + c] = sst;
     }
   };
 
-  pages(pc.tile);
+  next_page(pc.tile);
   Rows<D, NR> w;
   w.template load<false, PT>(s, pc, wr, c, g);
   fetch(pc.tile);
-  pages(pa_min(pc.tile + 1, pc.tile_end - 1));
+  next_page(pa_min(pc.tile + 1, pc.tile_end - 1));
   store(pc.tile, 0);
   if (pc.tile + 1 < pc.tile_end) fetch(pc.tile + 1);
-  pages(pa_min(pc.tile + 2, pc.tile_end - 1));
+  next_page(pa_min(pc.tile + 2, pc.tile_end - 1));
   __syncthreads();
   int buffer = 0;
   for (int tile = pc.tile; tile < pc.tile_end; ++tile, buffer ^= 1) {
-    const i32x4* lk = (const i32x4*)(lds + buffer * kBuffer);
-    const i32x4* lv = lk + SP_TILE * D / 8;
+    const i32x4* lk = (const i32x4*)(lds + buffer * tile_bytes(D));
+    const i32x4* lv = lk + D / 8 * kKeyRow;
     const float* lsc = (const float*)(lv + SP_TILE * D / 8);
     f32x4 x[NR][NT], vs[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
+    for (int k = 0; k < D / 32; ++k)  // NR NT sums side by side
 #pragma unroll
-      for (int n = 0; n < NR; ++n) x[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < NT; ++t) {
+        const i32x4 kf = lk[(4 * k + g) * kKeyRow + (wi * NT + t) * kKeyTile + c];
 #pragma unroll
-      for (int k = 0; k < D / 32; ++k) {
-        const i32x4 kf = lk[(4 * k + g) * SP_TILE + (wi * NT + t) * 16 + c];
-#pragma unroll
-        for (int n = 0; n < NR; ++n) x[n][t] = mfma<F16>(kf, w.q[n][k], x[n][t]);
+        for (int n = 0; n < NR; ++n) x[n][t] = mfma<F16>(kf, w.q[n][k], k ? x[n][t] : f32x4{0.f, 0.f, 0.f, 0.f});
       }
-    }
     if constexpr (PT) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -679,6 +750,7 @@ __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, cha
     }
     const int t0 = tile * SP_TILE;
     if (t0 < pc.begin || t0 + SP_TILE > pa_min(w.least, pc.end)) {
+      asm volatile("");  // (a branch: not computed for every tile)
 #pragma unroll
       for (int n = 0; n < NR; ++n)
 #pragma unroll
@@ -690,12 +762,11 @@ __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, cha
           }
     }
     i32x4 p[NR][NJ];
+    w.template softmax<PT, PF16, NT>(x, vs, p);
 #pragma unroll
-    for (int n = 0; n < NR; ++n) w.template softmax<PT, PF16, NT>(n, x[n], vs, p[n]);
+    for (int j = 0; j < NJ; ++j)
 #pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
+      for (int dt = 0; dt < D / 16; ++dt) {
         const i32x4 vf = lv[(2 * g + wi * NJ + j) * D + 16 * dt + c];
 #pragma unroll
         for (int n = 0; n < NR; ++n) w.o[n][dt] = mfma<PF16>(vf, p[n][j], w.o[n][dt]);
@@ -703,7 +774,7 @@ __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, cha
     if (tile + 1 < pc.tile_end) {
       store(tile + 1, buffer ^ 1);
       if (tile + 2 < pc.tile_end) fetch(tile + 2);
-      pages(pa_min(tile + 3, pc.tile_end - 1));
+      next_page(pa_min(tile + 3, pc.tile_end - 1));
     }
     __syncthreads();
   }
@@ -777,7 +848,7 @@ __global__ __launch_bounds__(kThreads, 2) void pa_shared_prefix_kernel(const SpA
       const int gr = group_of(pl, G, of);
       tiles = s.col_tiles;
       begin = gr >= 0 ? pl.len[gr] : 0;
-      end = context_of(s, of);
+      end = pl.ctx[of];
     }
     tiles = __builtin_amdgcn_readfirstlane(tiles);
     begin = __builtin_amdgcn_readfirstlane(begin);
