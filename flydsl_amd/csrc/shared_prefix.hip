@@ -63,7 +63,7 @@ struct SpArgs {
   pa_fp8_shared_prefix_args a;
   SpShape p, s;           // prefix and suffix items
   int eq, col_tiles;      // query columns per kv head, suffix items per (sequence, kv head)
-  int s_rows;             // rows a suffix piece stores
+  int p_rows, s_rows;     // rows a piece's slot has
   int capacity;           // tokens a table row can hold
   int lbs;                // log2(page size)
   // workspace
@@ -238,7 +238,7 @@ __device__ __forceinline__ void plan_group(const SpArgs& s, int sequences, int g
   const int rows = sequences * s.eq;
   *len = rows > 0 ? pa_min(pa_max(given, 0), s.capacity) : 0;
   *tiles = *len > 0 ? pa_cdiv(rows, s.p.rows) : 0;
-  *cost = (int64_t)*tiles * sp_item_cost(sp_steps(0, *len, s.p.tiles), s.p.cost);
+  *cost = (int64_t)*tiles * sp_item_cost(s.p, sp_tiles(0, *len));
 }
 
 // Every workgroup makes the whole plan: two rounds of loads (all lengths, then
@@ -293,7 +293,7 @@ __device__ void make_plan(const Plan& p, const SpArgs& s) {
   for (int b = threadIdx.x * per; b < pa_min((int)(threadIdx.x + 1) * per, B); ++b) {
     const int g = group_of(p, G, b);
     const int len = g >= 0 ? p.len[g] : 0;
-    p.seq_at[b] = (int64_t)s.col_tiles * sp_item_cost(sp_steps(len, p.ctx[b], s.s.tiles), s.s.cost);
+    p.seq_at[b] = (int64_t)s.col_tiles * sp_item_cost(s.s, sp_tiles(len, p.ctx[b]));
   }
   block_scan<false>(p.seq_at, B, p.scratch);
 }
@@ -313,8 +313,8 @@ struct Piece {
   float* o;
 };
 
-// LDS behind the plan: two buffers of a tile (run_shared), or, at a piece's end,
-// maxima and sums by wave and 32 output dims of every row.
+// LDS behind the plan, of shared items: two buffers of a tile, or, at a piece's
+// end, maxima and sums by wave and 32 output dims of every row.
 constexpr int kOutStride = 36;  // floats a row of 32 dims takes (16-byte steps that spread over the banks)
 __host__ __device__ constexpr int end_bytes(int nr) {
   return SP_WAVES * 16 * nr * 4 * 2 + SP_WAVES * 16 * nr * kOutStride * 4;
@@ -370,11 +370,10 @@ struct Rows {
     least = __builtin_amdgcn_readfirstlane(least);
   }
 
-  // Softmax of NT tiles' logits x (tokens t0 + 16 g + 4 (T0 + T) + i of the lane's
-  // row of each n) against the rows' references; p: the probabilities (times
-  // vs) as operands.
-  template <bool PT, bool PF16, int NT>
-  __device__ __forceinline__ void softmax(const f32x4 (&x)[NR][NT], const f32x4 (&vs)[NT], i32x4 (&p)[NR][NT / 2]) {
+  // Moves the rows' references to where logits x (of the lane's row of each n)
+  // need them.
+  template <int NT>
+  __device__ __forceinline__ void reference(const f32x4 (&x)[NR][NT]) {
     float top[NR];
     bool moves = false;
 #pragma unroll
@@ -398,24 +397,33 @@ struct Rows {
         m[n] = mn;
       }
     }
+  }
+
+  // Probabilities (times vs) of row n's logits of two key tiles, as an operand.
+  template <bool PT, bool PF16>
+  __device__ __forceinline__ i32x4 weights(int n, const f32x4& x0, const f32x4& x1, const f32x4& vs0, const f32x4& vs1) {
+    const float bias = m[n] == kNegInf ? 0.0f : -m[n];
+    float e[8], w[8];
 #pragma unroll
-    for (int n = 0; n < NR; ++n) {
-      const float bias = m[n] == kNegInf ? 0.0f : -m[n];
-      float w[4 * NT], sum = 0.0f;
-#pragma unroll
-      for (int T = 0; T < NT; ++T)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][T][i], fac, bias));
-          sum += e;
-          w[4 * T + i] = PT ? e * vs[T][i] : e;
-        }
-      l[n] += sum;
-#pragma unroll
-      for (int j = 0; j < NT / 2; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[n][j][i] = round2<PF16>(w[8 * j + 2 * i], w[8 * j + 2 * i + 1]);
+    for (int i = 0; i < 8; ++i) {
+      e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(i < 4 ? x0[i] : x1[i - 4], fac, bias));
+      w[i] = PT ? e[i] * (i < 4 ? vs0[i] : vs1[i - 4]) : e[i];
     }
+    l[n] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+    return i32x4{round2<PF16>(w[0], w[1]), round2<PF16>(w[2], w[3]), round2<PF16>(w[4], w[5]), round2<PF16>(w[6], w[7])};
+  }
+
+  // Writes a piece that one wave worked alone.
+  __device__ __forceinline__ void finish_alone(const Piece& pc, int c, int g) {
+    static_assert(NR == 1, "one row tile");
+    l[0] = groups_sum(l[0]);
+    if (pc.row0 + c >= pc.nrows) return;
+    if (g == 0) {
+      pc.ml[c] = m[0];
+      pc.ml[pc.rows_out + c] = l[0];
+    }
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) *(f32x4*)(pc.o + (int64_t)c * D + 16 * dt + 4 * g) = o[0][dt];
   }
 
   // Joins the waves of the same rows (wt of them, this one the wi-th) and writes
@@ -506,13 +514,12 @@ struct ScalarPages : Pages {
 };
 
 template <int D, bool F16, bool PT>
-__device__ __forceinline__ void run_direct(const SpArgs& s, const Piece& pc, char* lds) {
+__device__ __forceinline__ void run_direct(const SpArgs& s, const Piece& pc) {
   // the value product of f16 queries with per-token scales runs in bf16: a
   // scale of any size times a probability stays in range
   constexpr bool PF16 = F16 && !PT;
   const pa_fp8_shared_prefix_args& a = s.a;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int bs = 1 << s.lbs;
   const Pages page_of(s, pc);
   const uint8_t* kbase = (const uint8_t*)a.key_cache + (int64_t)pc.h * a.stride_k_head;
@@ -542,27 +549,23 @@ __device__ __forceinline__ void run_direct(const SpArgs& s, const Piece& pc, cha
     for (int T = 0; T < 4; ++T) x[T] = *(const f32x4*)(p + 4 * T);
   };
 
-  int tile = pc.tile + wave;
-  int kp = 0, vp = 0;
-  if (tile < pc.tile_end) {
-    kp = page_of(tile * SP_TILE + 16 * kblk);
-    vp = page_of(tile * SP_TILE + 16 * g);
-  }
+  int tile = pc.tile;
+  int kp = page_of(tile * SP_TILE + 16 * kblk), vp = page_of(tile * SP_TILE + 16 * g);
   Rows<D, 1> w;
   w.template load<true, PT>(s, pc, 0, c, g);
-  if (tile < pc.tile_end) {
-    load_keys(tile, kp);
-    load_values(tile, vp);
-    if constexpr (PT) {
-      load_scales(a.key_scale, tile, vp, ks);
-      load_scales(a.value_scale, tile, vp, vs);
-    }
-    const int next = pa_min(tile + SP_WAVES, pc.tile_end - 1);
+  load_keys(tile, kp);
+  load_values(tile, vp);
+  if constexpr (PT) {
+    load_scales(a.key_scale, tile, vp, ks);
+    load_scales(a.value_scale, tile, vp, vs);
+  }
+  {
+    const int next = pa_min(tile + 1, pc.tile_end - 1);
     kp = page_of(next * SP_TILE + 16 * kblk);
     vp = page_of(next * SP_TILE + 16 * g);
   }
-  for (; tile < pc.tile_end; tile += SP_WAVES) {
-    const int next = tile + SP_WAVES;
+  for (; tile < pc.tile_end; ++tile) {
+    const int next = tile + 1;
     const bool more = next < pc.tile_end;
     f32x4 x[1][4];
 #pragma unroll
@@ -609,23 +612,24 @@ __device__ __forceinline__ void run_direct(const SpArgs& s, const Piece& pc, cha
           }
       }
     }
-    i32x4 p[1][2];
-    w.template softmax<PT, PF16, 4>(x, vs, p);
+    w.reference(x);
+    const i32x4 p0 = w.template weights<PT, PF16>(0, x[0][0], x[0][1], vs[0], vs[1]);
+    const i32x4 p1 = w.template weights<PT, PF16>(0, x[0][2], x[0][3], vs[2], vs[3]);
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) {
       const i32x4 v0 = widen8<PF16>(vr[dt][0], vr[dt][1]), v1 = widen8<PF16>(vr[dt][2], vr[dt][3]);
-      w.o[0][dt] = mfma<PF16>(v0, p[0][0], w.o[0][dt]);
-      w.o[0][dt] = mfma<PF16>(v1, p[0][1], w.o[0][dt]);
+      w.o[0][dt] = mfma<PF16>(v0, p0, w.o[0][dt]);
+      w.o[0][dt] = mfma<PF16>(v1, p1, w.o[0][dt]);
     }
     if (more) {
       load_values(next, vp);
       if constexpr (PT) load_scales(a.value_scale, next, vp, vs);
-      const int after = pa_min(next + SP_WAVES, pc.tile_end - 1);
+      const int after = pa_min(next + 1, pc.tile_end - 1);
       kp = page_of(after * SP_TILE + 16 * kblk);
       vp = page_of(after * SP_TILE + 16 * g);
     }
   }
-  w.finish(pc, lds, SP_WAVES, wave, 0, wave, c, g);
+  w.finish_alone(pc, c, g);
 }
 
 // A tile in LDS, 16-byte pieces: keys [D / 8 octets of dims][64 rows of the key
@@ -639,8 +643,11 @@ __host__ __device__ constexpr int tile_bytes(int d) {
 }
 
 __host__ __device__ constexpr int work_bytes(int d, bool shared) {
-  return shared ? 2 * tile_bytes(d) : end_bytes(1);
+  return shared ? 2 * tile_bytes(d) : 0;
 }
+
+// Masks of the scheduling groups.
+constexpr int kSchedAlu = 0x2, kSchedMfma = 0x8, kSchedDsRead = 0x100;
 
 template <int D, bool F16, bool PT, int NR, int WT>
 __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, char* lds) {
@@ -730,15 +737,32 @@ __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, cha
     const i32x4* lk = (const i32x4*)(lds + buffer * tile_bytes(D));
     const i32x4* lv = lk + D / 8 * kKeyRow;
     const float* lsc = (const float*)(lv + SP_TILE * D / 8);
+    // Operand reads run a step ahead of the products, the first value product's
+    // behind the keys' (left to itself, the compiler waits out the latency of
+    // every read).
+    constexpr int K = D / 32, VA = D / 16, VP = VA / 2;
     f32x4 x[NR][NT], vs[NT];
+    i32x4 kf[K][NT], vf[VA];
+    auto read_keys = [&](int k) {
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k)  // NR NT sums side by side
+      for (int t = 0; t < NT; ++t) kf[k][t] = lk[(4 * k + g) * kKeyRow + (wi * NT + t) * kKeyTile + c];
+    };
+    read_keys(0);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const i32x4 kf = lk[(4 * k + g) * kKeyRow + (wi * NT + t) * kKeyTile + c];
+    for (int k = 0; k < K; ++k) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (k + 1 < K) {
+        read_keys(k + 1);
+      } else {
 #pragma unroll
-        for (int n = 0; n < NR; ++n) x[n][t] = mfma<F16>(kf, w.q[n][k], k ? x[n][t] : f32x4{0.f, 0.f, 0.f, 0.f});
+        for (int dt = 0; dt < VP; ++dt) vf[dt] = lv[(2 * g + wi * NJ) * D + 16 * dt + c];
       }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int n = 0; n < NR; ++n) x[n][t] = mfma<F16>(kf[k][t], w.q[n][k], k ? x[n][t] : f32x4{0.f, 0.f, 0.f, 0.f});
+    }
+    __builtin_amdgcn_sched_barrier(0);
     if constexpr (PT) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -761,16 +785,46 @@ __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, cha
             if (at < pc.begin || at >= w.limit[n]) x[n][t][i] = kNegInf;
           }
     }
-    i32x4 p[NR][NJ];
-    w.template softmax<PT, PF16, NT>(x, vs, p);
+    w.reference(x);
+    i32x4 p[NR];
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
+    for (int n = 0; n < NR; ++n) p[n] = w.template weights<PT, PF16>(n, x[n][0], x[n][1], vs[0], vs[1]);
+    // the first product beside the second half's probabilities, reads VP ahead
+    __builtin_amdgcn_sched_barrier(0);
+    i32x4 p1[NR], vf1[VA];
+    if constexpr (NJ == 2) {
 #pragma unroll
-      for (int dt = 0; dt < D / 16; ++dt) {
-        const i32x4 vf = lv[(2 * g + wi * NJ + j) * D + 16 * dt + c];
+      for (int n = 0; n < NR; ++n) p1[n] = w.template weights<PT, PF16>(n, x[n][2], x[n][3], vs[2], vs[3]);
+    }
 #pragma unroll
-        for (int n = 0; n < NR; ++n) w.o[n][dt] = mfma<PF16>(vf, p[n][j], w.o[n][dt]);
+    for (int i = VP; i < VP + VA; ++i) {
+      if (i < VA)
+        vf[i] = lv[(2 * g + wi * NJ) * D + 16 * i + c];
+      else if (NJ == 2)
+        vf1[i - VA] = lv[(2 * g + 1) * D + 16 * (i - VA) + c];
+#pragma unroll
+      for (int n = 0; n < NR; ++n) w.o[n][i - VP] = mfma<PF16>(vf[i - VP], p[n], w.o[n][i - VP]);
+    }
+#pragma unroll
+    for (int dt = 0; dt < VA; ++dt) {
+      __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kSchedMfma, NR, 0);
+      if (NJ == 2) __builtin_amdgcn_sched_group_barrier(kSchedAlu, (PT ? 40 : 32) * NR * 16 / D, 0);
+    }
+    if constexpr (NJ == 2) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = VP; i < VP + VA; ++i) {
+        if (i < VA) vf1[i] = lv[(2 * g + 1) * D + 16 * i + c];
+#pragma unroll
+        for (int n = 0; n < NR; ++n) w.o[n][i - VP] = mfma<PF16>(vf1[i - VP], p1[n], w.o[n][i - VP]);
       }
+#pragma unroll
+      for (int dt = 0; dt < VA; ++dt) {
+        __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kSchedMfma, NR, 0);
+      }
+    }
     if (tile + 1 < pc.tile_end) {
       store(tile + 1, buffer ^ 1);
       if (tile + 2 < pc.tile_end) fetch(tile + 2);
@@ -781,26 +835,100 @@ __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, cha
   w.finish(pc, lds, WT, wave, wr, wi, c, g);
 }
 
-template <int D, bool F16, bool PT>
-__device__ __forceinline__ void run_piece(const SpArgs& s, const SpShape& sh, const Piece& pc, char* lds) {
-  constexpr int most = D <= 128 ? 2 : 1;
-  if constexpr (D <= 128) {
-    if (!sh.shared) {
-      run_direct<D, F16, PT>(s, pc, lds);
-      return;
-    }
-  }
-  if (sh.wt == 1)
-    run_shared<D, F16, PT, most, 1>(s, pc, lds);
-  else if (most == 1 || sh.nr == 1)
-    run_shared<D, F16, PT, 1, 2>(s, pc, lds);
-  else
-    run_shared<D, F16, PT, most, 2>(s, pc, lds);
-}
+static_assert(end_bytes(2) <= 2 * tile_bytes(64), "a piece's end fits the tiles' buffers");
 
 // ---------------------------------------------------------------------------
 // The kernels
 // ---------------------------------------------------------------------------
+
+// Works the tiles of the line's region [from, to) that begin in [lo, hi) (the
+// share of `worker`, as long as `share`): a workgroup's (WAVE false) or a wave's.
+template <int D, bool F16, bool PT, bool WAVE>
+__device__ __forceinline__ void walk(const SpArgs& s, const Plan& pl, int64_t prefix_line, int64_t from, int64_t to,
+                                     int64_t lo, int64_t hi, int64_t share, int worker, char* work) {
+  const int B = s.a.num_seqs, G = s.a.num_groups, H = s.a.num_kv_heads;
+  const int64_t start = lo > from ? lo : from, stop = hi < to ? hi : to;
+  if (start >= stop) return;
+  // The item that holds position `start`, then those behind it: `of` a group or a
+  // sequence, `idx` the item among its own (kv head outer, row tile inner).
+  bool prefix = start < prefix_line;
+  int of = __builtin_amdgcn_readfirstlane(prefix ? last_le(pl.group_at, G, start, H)
+                                                 : last_le(pl.seq_at, B, start - prefix_line, H));
+  int idx = -1;
+  int64_t at = 0;  // of item idx
+  while (true) {
+    const SpShape& sh = prefix ? s.p : s.s;
+    int begin, end, tiles;
+    if (prefix) {
+      tiles = pl.row_tiles[of + 1] - pl.row_tiles[of];
+      begin = 0;
+      end = pl.len[of];
+    } else {
+      const int gr = group_of(pl, G, of);
+      tiles = s.col_tiles;
+      begin = gr >= 0 ? pl.len[gr] : 0;
+      end = pl.ctx[of];
+    }
+    tiles = __builtin_amdgcn_readfirstlane(tiles);
+    begin = __builtin_amdgcn_readfirstlane(begin);
+    end = __builtin_amdgcn_readfirstlane(end);
+    const int n = sp_tiles(begin, end), cost = sp_item_cost(sh, n);
+    if (idx < 0) {  // the first one
+      const int64_t of_at = prefix ? (int64_t)H * pl.group_at[of] : prefix_line + (int64_t)H * pl.seq_at[of];
+      idx = __builtin_amdgcn_readfirstlane(sp_worker_of(start - of_at, cost));
+      at = of_at + (int64_t)idx * cost;
+    }
+    for (; idx < H * tiles && at < stop; ++idx, at += cost) {
+      const int t0 = __builtin_amdgcn_readfirstlane(sp_tile_from(sh, lo, at, n));
+      const int t1 = __builtin_amdgcn_readfirstlane(sp_tile_from(sh, hi, at, n));
+      if (t1 <= t0) continue;
+      const int item = __builtin_amdgcn_readfirstlane(prefix ? H * pl.row_tiles[of] + idx : of * H * tiles + idx);
+      const int h = idx / tiles, slot = item + worker;
+      Piece pc;
+      pc.b0 = prefix ? __builtin_amdgcn_readfirstlane(pl.first[of]) : of;
+      pc.h = h;
+      pc.row0 = (idx - h * tiles) * sh.rows;
+      pc.nrows = prefix ? __builtin_amdgcn_readfirstlane((pl.first[of + 1] - pl.first[of]) * s.eq) : s.eq;
+      pc.begin = begin;
+      pc.end = end;
+      pc.tile = begin / SP_TILE + t0;
+      pc.tile_end = begin / SP_TILE + t1;
+      pc.rows_out = prefix ? s.p_rows : s.s_rows;
+      pc.ml = (prefix ? s.p_ml : s.s_ml) + (int64_t)slot * 2 * pc.rows_out;
+      pc.o = (prefix ? s.p_o : s.s_o) + (int64_t)slot * pc.rows_out * D;
+      if (t0 == 0 && (WAVE ? (threadIdx.x & 63) : threadIdx.x) == 0) {
+        const int last = sp_worker_of(at + sh.overhead + (int64_t)(n - 1) * sh.cost, share);
+        s.items[prefix ? item : s.max_prefix_items + item] = int2{slot, last - worker + 1};
+      }
+      if constexpr (WAVE) {
+        run_direct<D, F16, PT>(s, pc);
+      } else {
+        constexpr int most = D <= 128 ? 2 : 1;
+        if (sh.wt == 1)
+          run_shared<D, F16, PT, most, 1>(s, pc, work);
+        else if (most == 1 || sh.nr == 1)
+          run_shared<D, F16, PT, 1, 2>(s, pc, work);
+        else
+          run_shared<D, F16, PT, most, 2>(s, pc, work);
+      }
+    }
+    if (at >= stop) return;
+    // on to the next group or sequence that has items
+    idx = 0;
+    ++of;
+    if (prefix) {
+      while (of < G && pl.group_at[of + 1] == pl.group_at[of]) ++of;
+      if (of >= G) {
+        prefix = false;
+        of = 0;
+      }
+    }
+    if (!prefix)
+      while (of < B && pl.seq_at[of + 1] == pl.seq_at[of]) ++of;
+    if (!prefix && of >= B) return;
+    of = __builtin_amdgcn_readfirstlane(of);
+  }
+}
 
 template <int D, bool F16, bool PT>
 __global__ __launch_bounds__(kThreads, 2) void pa_shared_prefix_kernel(const SpArgs s) {
@@ -828,77 +956,15 @@ __global__ __launch_bounds__(kThreads, 2) void pa_shared_prefix_kernel(const SpA
   const int64_t share = sp_share(line, gridDim.x);
   const int64_t lo = (int64_t)worker * share;
   if (lo >= line) return;
-  const int64_t hi = lo + share < line ? lo + share : line;
-
-  // The item that holds position lo, then those behind it: `of` a group or a
-  // sequence, `idx` the item among its own (kv head outer, row tile inner).
-  bool prefix = lo < prefix_line;
-  int of = __builtin_amdgcn_readfirstlane(prefix ? last_le(pl.group_at, G, lo, H)
-                                                 : last_le(pl.seq_at, B, lo - prefix_line, H));
-  int idx = -1;
-  int64_t at = 0;  // of item idx
-  while (true) {
-    const SpShape& sh = prefix ? s.p : s.s;
-    int begin, end, tiles;
-    if (prefix) {
-      tiles = pl.row_tiles[of + 1] - pl.row_tiles[of];
-      begin = 0;
-      end = pl.len[of];
-    } else {
-      const int gr = group_of(pl, G, of);
-      tiles = s.col_tiles;
-      begin = gr >= 0 ? pl.len[gr] : 0;
-      end = pl.ctx[of];
-    }
-    tiles = __builtin_amdgcn_readfirstlane(tiles);
-    begin = __builtin_amdgcn_readfirstlane(begin);
-    end = __builtin_amdgcn_readfirstlane(end);
-    const int steps = sp_steps(begin, end, sh.tiles);
-    const int cost = sp_item_cost(steps, sh.cost);
-    const int64_t of_at = prefix ? (int64_t)H * pl.group_at[of] : prefix_line + (int64_t)H * pl.seq_at[of];
-    if (idx < 0) {  // the first one
-      idx = sp_worker_of(lo - of_at, cost);
-      at = of_at + (int64_t)idx * cost;
-    }
-    for (; idx < H * tiles && at < hi; ++idx, at += cost) {
-      const int s0 = sp_step_from(lo, at, steps, sh.cost), s1 = sp_step_from(hi, at, steps, sh.cost);
-      if (s1 <= s0) continue;
-      const int item = prefix ? H * pl.row_tiles[of] + idx : of * H * tiles + idx;
-      const int t0 = begin / SP_TILE, h = idx / tiles;
-      const int slot = __builtin_amdgcn_readfirstlane(item + worker);
-      Piece pc;
-      pc.b0 = prefix ? __builtin_amdgcn_readfirstlane(pl.first[of]) : of;
-      pc.h = __builtin_amdgcn_readfirstlane(h);
-      pc.row0 = __builtin_amdgcn_readfirstlane((idx - h * tiles) * sh.rows);
-      pc.nrows = prefix ? __builtin_amdgcn_readfirstlane((pl.first[of + 1] - pl.first[of]) * s.eq) : s.eq;
-      pc.begin = begin;
-      pc.end = end;
-      pc.tile = __builtin_amdgcn_readfirstlane(t0 + s0 * sh.tiles);
-      pc.tile_end = __builtin_amdgcn_readfirstlane(pa_min(t0 + s1 * sh.tiles, pa_cdiv(end, SP_TILE)));
-      pc.rows_out = prefix ? s.p.rows : s.s_rows;
-      pc.ml = (prefix ? s.p_ml : s.s_ml) + (int64_t)slot * 2 * pc.rows_out;
-      pc.o = (prefix ? s.p_o : s.s_o) + (int64_t)slot * pc.rows_out * D;
-      if (s0 == 0 && threadIdx.x == 0) {
-        const int last = sp_worker_of(at + SP_OVERHEAD + (int64_t)(steps - 1) * sh.cost, share);
-        s.items[prefix ? item : s.max_prefix_items + item] = int2{item + worker, last - worker + 1};
-      }
-      run_piece<D, F16, PT>(s, sh, pc, work);
-    }
-    if (at >= hi) return;
-    // on to the next group or sequence that has items
-    idx = 0;
-    ++of;
-    if (prefix) {
-      while (of < G && pl.group_at[of + 1] == pl.group_at[of]) ++of;
-      if (of >= G) {
-        prefix = false;
-        of = 0;
-      }
-    }
-    if (!prefix)
-      while (of < B && pl.seq_at[of + 1] == pl.seq_at[of]) ++of;
-    if (!prefix && of >= B) return;
-    of = __builtin_amdgcn_readfirstlane(of);
+  // shared items first, the workgroup together (prefix items have at least a
+  // suffix item's rows, so direct prefix items mean direct suffix items)
+  const int64_t shared_line = s.s.shared ? line : (s.p.shared ? prefix_line : 0);
+  walk<D, F16, PT, false>(s, pl, prefix_line, 0, shared_line, lo, lo + share, share, worker, work);
+  if constexpr (D <= 128) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t quarter = share / SP_WAVES, wlo = lo + wave * quarter;
+    walk<D, F16, PT, true>(s, pl, prefix_line, shared_line, line, wlo, wlo + quarter, quarter, worker * SP_WAVES + wave,
+                           nullptr);
   }
 }
 
@@ -941,7 +1007,7 @@ __global__ __launch_bounds__(kMergeThreads) void pa_shared_prefix_merge_kernel(c
     if (info.x >= 0) {
       const int row = info.y + e, t = row / s.p.rows;
       const int2 it = s.items[info.x + h * info.z + t];
-      take(s.p_ml, s.p_o, s.p.rows, it.x, it.y, row - t * s.p.rows);
+      take(s.p_ml, s.p_o, s.p_rows, it.x, it.y, row - t * s.p.rows);
     }
     if (info.w) {
       const int t = e / s.s.rows;
@@ -1006,17 +1072,18 @@ int sizes_of(int B, int G, int H, int ql, int gqa, int D, int workers, Sizes* z)
   z->s = sp_shape((int)eq, D);
   z->col_tiles = (int)((eq + z->s.rows - 1) / z->s.rows);
   z->s_rows = z->col_tiles > 1 ? z->s.rows : (int)eq;
-  z->p = sp_shape((int)((rows + pa_max(G, 1) - 1) / pa_max(G, 1)), D);
+  z->p = sp_shape(pa_max((int)((rows + pa_max(G, 1) - 1) / pa_max(G, 1)), z->eq), D);
   z->prefix_items = G > 0 ? (rows / z->p.rows + pa_min(G, B)) * H : 0;
   z->suffix_items = (int64_t)B * H * z->col_tiles;
-  if (z->prefix_items + workers > 0x7fffffff / 2 || z->suffix_items + workers > 0x7fffffff / 2) return PA_ERR_SHAPE;
+  if (workers > (1 << 20) || z->prefix_items > 0x3fffffff || z->suffix_items > 0x3fffffff) return PA_ERR_SHAPE;
   int64_t at = 0;
   auto take = [&](int64_t n) {
     const int64_t here = at;
     at = (at + n + 255) & ~(int64_t)255;
     return here;
   };
-  const int64_t np = z->prefix_items > 0 ? z->prefix_items + workers : 0, ns = z->suffix_items + workers;
+  const int64_t np = z->prefix_items > 0 ? z->prefix_items + workers * (z->p.shared ? 1 : SP_WAVES) : 0;
+  const int64_t ns = z->suffix_items + workers * (z->s.shared ? 1 : SP_WAVES);
   z->seq_info = take(16 * (int64_t)B);
   z->items = take(8 * (z->prefix_items + z->suffix_items));
   z->p_ml = take(np * 8 * z->p.rows);
@@ -1077,7 +1144,7 @@ extern "C" int pa_fp8_plan_shared_prefix(const int32_t* context_lengths, const i
   for (int g = 0; g <= G && G > 0; ++g) first[g] = top = pa_max(top, pa_min(pa_max(prefix_indptr[g], 0), B));
   struct Kind {
     bool prefix;
-    int of, h0, items, begin, steps, end, base;
+    int of, h0, items, begin, tiles, base;
   };
   std::vector<Kind> line;
   int64_t total = 0;
@@ -1086,15 +1153,15 @@ extern "C" int pa_fp8_plan_shared_prefix(const int32_t* context_lengths, const i
     len[g] = rows > 0 ? pa_min(pa_max(prefix_lengths[g], 0), capacity) : 0;
     for (int b = first[g]; b < first[g + 1]; ++b) seq_len[b] = len[g];
     tiles[g + 1] = tiles[g] + (len[g] > 0 ? pa_cdiv(rows, z.p.rows) : 0);
-    const int n = tiles[g + 1] - tiles[g], steps = sp_steps(0, len[g], z.p.tiles);
-    if (n > 0) line.push_back({true, g, n, H * n, 0, steps, len[g], H * tiles[g]});
-    total += (int64_t)H * n * sp_item_cost(steps, z.p.cost);
+    const int n = tiles[g + 1] - tiles[g], steps = sp_tiles(0, len[g]);
+    if (n > 0) line.push_back({true, g, n, H * n, 0, steps, H * tiles[g]});
+    total += (int64_t)H * n * sp_item_cost(z.p, steps);
   }
   for (int b = 0; b < B; ++b) {
     const int end = pa_min(pa_max(context_lengths[b], 0), capacity);
-    const int steps = sp_steps(seq_len[b], end, z.s.tiles);
-    if (steps > 0) line.push_back({false, b, z.col_tiles, H * z.col_tiles, seq_len[b], steps, end, b * H * z.col_tiles});
-    total += (int64_t)H * z.col_tiles * sp_item_cost(steps, z.s.cost);
+    const int steps = sp_tiles(seq_len[b], end);
+    if (steps > 0) line.push_back({false, b, z.col_tiles, H * z.col_tiles, seq_len[b], steps, b * H * z.col_tiles});
+    total += (int64_t)H * z.col_tiles * sp_item_cost(z.s, steps);
   }
   if (total == 0) return 0;
   const int64_t share = sp_share(total, workers);
@@ -1102,21 +1169,18 @@ extern "C" int pa_fp8_plan_shared_prefix(const int32_t* context_lengths, const i
   int64_t at = 0;
   for (const Kind& k : line) {
     const SpShape& sh = k.prefix ? z.p : z.s;
+    const int64_t q = sh.shared ? share : share / SP_WAVES;
     for (int i = 0; i < k.items; ++i) {
-      const int w0 = sp_worker_of(at + SP_OVERHEAD, share);
-      const int w1 = sp_worker_of(at + SP_OVERHEAD + (int64_t)(k.steps - 1) * sh.cost, share);
+      const int w0 = sp_worker_of(at + sh.overhead, q);
+      const int w1 = sp_worker_of(at + sh.overhead + (int64_t)(k.tiles - 1) * sh.cost, q);
       for (int w = w0; w <= w1; ++w) {
-        const int s0 = sp_step_from(w * share, at, k.steps, sh.cost);
-        const int s1 = sp_step_from((w + 1) * share, at, k.steps, sh.cost);
-        if (n < max_pieces) {
-          const int t0 = k.begin / SP_TILE;
-          const int32_t rec[8] = {k.prefix, k.base + i, w, k.base + i + w, k.of, i / k.h0, t0 + s0 * sh.tiles,
-                                  pa_min(t0 + s1 * sh.tiles, pa_cdiv(k.end, SP_TILE))};
-          for (int j = 0; j < 8; ++j) pieces[8 * n + j] = rec[j];
-        }
+        const int t0 = k.begin / SP_TILE + sp_tile_from(sh, w * q, at, k.tiles);
+        const int t1 = k.begin / SP_TILE + sp_tile_from(sh, (w + 1) * q, at, k.tiles);
+        const int32_t rec[8] = {k.prefix, k.base + i, w, k.base + i + w, k.of, i / k.h0, t0, t1};
+        for (int j = 0; j < 8 && n < max_pieces; ++j) pieces[8 * n + j] = rec[j];
         ++n;
       }
-      at += sp_item_cost(k.steps, sh.cost);
+      at += sp_item_cost(sh, k.tiles);
     }
   }
   return n;
@@ -1156,9 +1220,10 @@ extern "C" int pa_fp8_decode_shared_prefix(const pa_fp8_shared_prefix_args* a, v
   s.s = z.s;
   s.eq = z.eq;
   s.col_tiles = z.col_tiles;
+  s.p_rows = z.p.rows;
   s.s_rows = z.s_rows;
   const int64_t cap = (int64_t)a->max_blocks_per_seq * bs;
-  s.capacity = cap < (1 << 30) ? (int)cap : 1 << 30;
+  s.capacity = cap < SP_MAX_TOKENS ? (int)cap : SP_MAX_TOKENS;
   s.lbs = 31 - __builtin_clz((unsigned)bs);
   char* ws = (char*)workspace;
   s.seq_info = (int4*)(ws + z.seq_info);

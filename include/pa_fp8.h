@@ -679,8 +679,9 @@ int pa_fp8_decode_shared_prefix(const pa_fp8_shared_prefix_args* args, void* wor
                                 void* hip_stream);
 /*
  * The pieces those launches work, on the host: records of eight int32 (1 for a
- * prefix piece or 0, item, worker, slot, group or sequence, kv head, first
- * tile, end tile; tiles of 64 tokens) in the order of the line, at most
+ * prefix piece or 0, item, worker (a workgroup or, where one wave works an item
+ * alone, a wave), slot, group or sequence, kv head, first tile, end tile; tiles
+ * of 64 tokens) in the order of the line, at most
  * max_pieces of them.  Returns their number or a PA_ERR_* code.
  */
 int pa_fp8_plan_shared_prefix(const int32_t* context_lengths, const int32_t* prefix_indptr,

@@ -27,7 +27,8 @@ def check(ctx, indptr, prefix, hkv, ql, gqa, d, capacity, workers):
     first = np.maximum.accumulate(np.clip(indptr, 0, B)) if G else np.zeros(1, int)
     own = [0] * B
     want = {}  # (prefix, item) -> (of, head, first tile, end tile)
-    p_rows, s_rows = rows_of(-(-B * eq // max(G, 1)), d), rows_of(eq, d)
+    p_rows, s_rows = rows_of(max(-(-B * eq // max(G, 1)), eq), d), rows_of(eq, d)
+    most = [workers * (4 if r == 16 else 1) for r in (s_rows, p_rows)]  # a wave alone, or a workgroup
     item = 0
     for g in range(G):
         rows = (first[g + 1] - first[g]) * eq
@@ -49,8 +50,8 @@ def check(ctx, indptr, prefix, hkv, ql, gqa, d, capacity, workers):
                 want[0, b * hkv * ct + i] = (b, i // ct, own[b] // TILE, -(-n // TILE))
     got, slots = {}, set()
     for is_p, it, w, slot, of, h, t0, t1 in pieces.tolist():
-        assert t1 > t0 and 0 <= w < workers
-        assert (is_p, slot) not in slots and 0 <= slot < (bound if is_p else B * hkv * ct) + workers
+        assert t1 > t0 and 0 <= w < most[is_p]
+        assert (is_p, slot) not in slots and 0 <= slot < (bound if is_p else B * hkv * ct) + most[is_p]
         slots.add((is_p, slot))
         got.setdefault((is_p, it), []).append((of, h, t0, t1, w, slot))
     assert got.keys() == want.keys()
@@ -106,12 +107,13 @@ def test_lengths_are_held_to_a_table_row():
 
 
 def test_shares_are_even():
-    """On a long line no worker gets more than a step beyond the mean."""
+    """On a long line no workgroup gets more than a tile and a piece's overhead
+    beyond the mean."""
     pieces = check([17000 + i for i in range(256)], [0, 256], [16383], 8, 1, 4, 128, 1 << 20, 256)
     cost = np.zeros(256)
     for is_p, _, w, _, _, _, t0, t1 in pieces.tolist():
-        cost[w] += 6 + ((t1 - t0) * 4 if is_p else -(-(t1 - t0) // 4) * 8)
-    assert cost.max() <= cost.mean() + 8 + 12
+        cost[w if is_p else w // 4] += 120 + (t1 - t0) * 60 if is_p else 24 + (t1 - t0) * 8
+    assert cost.max() <= cost.mean() + 60 + 120
 
 
 def test_refusals():
