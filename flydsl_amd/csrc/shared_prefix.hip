@@ -53,10 +53,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr int kThreads = 64 * SP_WAVES;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_inff();
-// A row's reference exponent moves when a logit exceeds it by more than
-// this (base 2): the probabilities stay below 2^8, and most tiles leave the
-// accumulators as they are.
-constexpr float kRescaleMargin = 8.f;
+// A row's reference exponent starts below every logit.
+constexpr float kNoKey = -3.0e38f;
 
 // Everything a launch needs (device side of pa_fp8_shared_prefix_args).
 struct SpArgs {
@@ -71,6 +69,7 @@ struct SpArgs {
                           // row tiles of the group, whether the sequence has a suffix
   int2* items;            // [prefix items, then suffix items]: first slot, pieces
   int max_prefix_items;
+  int prefix_items;       // as many as an even split of the batch over the groups would make
   float* p_ml;            // [slot][2][rows]
   float* p_o;             // [slot][rows][D]
   float* s_ml;
@@ -148,13 +147,14 @@ struct Plan {
   int64_t* group_at;  // [G + 1] likewise of the groups' prefix items
   int64_t* scratch;   // [SP_WAVES]
   int* ctx;           // [B] context length, at most what a table row holds
+  int* begin;         // [B] prefix length of its group
   int* first;         // [G + 1] first sequence of a group (never falls)
   int* len;           // [G + 1] prefix length
   int* row_tiles;     // [G + 1] prefix items of the groups before g, one kv head
 };
 
 __host__ __device__ inline int plan_bytes(int B, int G) {
-  return (8 * (B + 1) + 8 * (G + 1) + 8 * SP_WAVES + 4 * B + 12 * (G + 1) + 15) & ~15;
+  return (8 * (B + 1) + 8 * (G + 1) + 8 * SP_WAVES + 8 * B + 12 * (G + 1) + 15) & ~15;
 }
 __device__ __forceinline__ Plan plan_of(char* lds, int B, int G) {
   Plan p;
@@ -162,7 +162,8 @@ __device__ __forceinline__ Plan plan_of(char* lds, int B, int G) {
   p.group_at = p.seq_at + B + 1;
   p.scratch = p.group_at + G + 1;
   p.ctx = (int*)(p.scratch + SP_WAVES);
-  p.first = p.ctx + B;
+  p.begin = p.ctx + B;
+  p.first = p.begin + B;
   p.len = p.first + G + 1;
   p.row_tiles = p.len + G + 1;
   return p;
@@ -245,6 +246,11 @@ __device__ __forceinline__ void plan_group(const SpArgs& s, int sequences, int g
 // none) and a few barriers, 1 us, where a launch of its own would take 3.
 __device__ void make_plan(const Plan& p, const SpArgs& s) {
   const int B = s.a.num_seqs, G = s.a.num_groups;
+  int f = 0, given = 0;  // asked for before anything waits
+  if (threadIdx.x < 64 && G < 64) {
+    if (G > 0 && (int)threadIdx.x <= G) f = s.a.prefix_indptr[threadIdx.x];
+    if ((int)threadIdx.x < G) given = s.a.prefix_lengths[threadIdx.x];
+  }
   for (int b = threadIdx.x; b < B; b += kThreads) {
     const int n = s.a.context_lengths[b];
     p.ctx[b] = n < 0 ? 0 : (n < s.capacity ? n : s.capacity);
@@ -252,10 +258,7 @@ __device__ void make_plan(const Plan& p, const SpArgs& s) {
   if (G < 64) {  // the groups in one wave's lanes
     if (threadIdx.x < 64) {
       const int g = threadIdx.x;
-      int f = 0, given = 0;
-      if (G > 0 && g <= G) f = pa_min(pa_max(s.a.prefix_indptr[g], 0), B);
-      if (g < G) given = s.a.prefix_lengths[g];
-      f = wave_upto<true>(f);
+      f = wave_upto<true>(pa_min(pa_max(f, 0), B));
       const int next = __shfl_down(f, 1, 64);
       int len = 0, tiles = 0;
       int64_t cost = 0;
@@ -293,6 +296,7 @@ __device__ void make_plan(const Plan& p, const SpArgs& s) {
   for (int b = threadIdx.x * per; b < pa_min((int)(threadIdx.x + 1) * per, B); ++b) {
     const int g = group_of(p, G, b);
     const int len = g >= 0 ? p.len[g] : 0;
+    p.begin[b] = len;
     p.seq_at[b] = (int64_t)s.col_tiles * sp_item_cost(s.s, sp_tiles(len, p.ctx[b]));
   }
   block_scan<false>(p.seq_at, B, p.scratch);
@@ -303,6 +307,7 @@ __device__ void make_plan(const Plan& p, const SpArgs& s) {
 // ---------------------------------------------------------------------------
 
 struct Piece {
+  bool of_prefix;     // a prefix item's
   int b0;            // sequence whose table row gives the pages, and of the item's row 0
   int row0, nrows;   // first row of the item among the group's rows (the sequence's columns), and their count
   int h;             // kv head
@@ -311,6 +316,111 @@ struct Piece {
   int rows_out;      // rows of a slot
   float* ml;         // the slot
   float* o;
+};
+
+// The pieces of the line's region [from, to) whose tiles begin in [lo, hi), the
+// part of `worker`, as long as `share`: a workgroup's or a wave's.
+struct Walk {
+  int64_t suffix_at, lo, hi, stop, share, at;  // suffix_at: where the suffix items begin; at: of item idx
+  int worker, of, idx;                           // `of` a group or a sequence, idx the item among its own (kv head
+                                                 // outer, row tile inner); -1: not looked up yet; INT_MAX: no more
+  bool prefix;
+
+  __device__ __forceinline__ void start(const SpArgs& s, const Plan& pl, int64_t suffix_at_, int64_t from, int64_t to,
+                                        int64_t lo_, int64_t share_, int worker_) {
+    suffix_at = suffix_at_;
+    lo = lo_;
+    share = share_;
+    hi = lo + share;
+    worker = worker_;
+    at = lo > from ? lo : from;
+    stop = hi < to ? hi : to;
+    idx = -1;
+    of = 0;
+    const int H = s.a.num_kv_heads;
+    prefix = at < (int64_t)H * pl.group_at[s.a.num_groups];
+    if (at >= stop) {
+      idx = 0x7fffffff;
+      return;
+    }
+    of = __builtin_amdgcn_readfirstlane(prefix ? last_le(pl.group_at, s.a.num_groups, at, H)
+                                               : last_le(pl.seq_at, s.a.num_seqs, at - suffix_at, H));
+  }
+
+  // The next piece; false when there is none.  ALONE: a wave's (its lane 0 tells
+  // the merge of it).
+  __device__ __forceinline__ bool next_piece(const SpArgs& s, const Plan& pl, int D, bool alone, Piece& pc) {
+    const int B = s.a.num_seqs, G = s.a.num_groups, H = s.a.num_kv_heads;
+    while (idx != 0x7fffffff) {
+      const SpShape& sh = prefix ? s.p : s.s;
+      int begin = 0, end, tiles;
+      if (prefix) {
+        tiles = pl.row_tiles[of + 1] - pl.row_tiles[of];
+        end = pl.len[of];
+      } else {
+        tiles = s.col_tiles;
+        begin = pl.begin[of];
+        end = pl.ctx[of];
+      }
+      tiles = __builtin_amdgcn_readfirstlane(tiles);
+      begin = __builtin_amdgcn_readfirstlane(begin);
+      end = __builtin_amdgcn_readfirstlane(end);
+      const int n = sp_tiles(begin, end), cost = sp_item_cost(sh, n);
+      if (idx < 0) {
+        const int64_t of_at = prefix ? (int64_t)H * pl.group_at[of] : suffix_at + (int64_t)H * pl.seq_at[of];
+        idx = __builtin_amdgcn_readfirstlane(sp_worker_of(at - of_at, cost));
+        at = of_at + (int64_t)idx * cost;
+      }
+      while (idx < H * tiles && at < stop) {
+        // (no division for an item that lies inside the part)
+        const int t0 = at + sh.overhead >= lo ? 0 : __builtin_amdgcn_readfirstlane(sp_tile_from(sh, lo, at, n));
+        const int t1 = at + cost <= hi ? n : __builtin_amdgcn_readfirstlane(sp_tile_from(sh, hi, at, n));
+        const int i = idx;
+        const int64_t i_at = at;
+        ++idx;
+        at += cost;
+        if (t1 <= t0) continue;
+        const int item = __builtin_amdgcn_readfirstlane(prefix ? H * pl.row_tiles[of] + i : of * H * tiles + i);
+        const int slot = item + worker;
+        pc.of_prefix = prefix;
+        pc.b0 = prefix ? __builtin_amdgcn_readfirstlane(pl.first[of]) : of;
+        pc.h = tiles == 1 ? i : i / tiles;
+        pc.row0 = (i - pc.h * tiles) * sh.rows;
+        pc.nrows = prefix ? __builtin_amdgcn_readfirstlane((pl.first[of + 1] - pl.first[of]) * s.eq) : s.eq;
+        pc.begin = begin;
+        pc.end = end;
+        pc.tile = begin / SP_TILE + t0;
+        pc.tile_end = begin / SP_TILE + t1;
+        pc.rows_out = prefix ? s.p_rows : s.s_rows;
+        pc.ml = (prefix ? s.p_ml : s.s_ml) + (int64_t)slot * 2 * pc.rows_out;
+        pc.o = (prefix ? s.p_o : s.s_o) + (int64_t)slot * pc.rows_out * D;
+        if (t0 == 0 && (alone ? (threadIdx.x & 63) : threadIdx.x) == 0) {
+          const int last = t1 == n ? worker : sp_worker_of(i_at + sh.overhead + ((int64_t)(n - 1) << sh.lcost), share);
+          s.items[prefix ? item : s.max_prefix_items + item] = int2{slot, last - worker + 1};
+        }
+        return true;
+      }
+      if (at >= stop) break;
+      // on to the next group or sequence that has items
+      idx = 0;
+      ++of;
+      if (prefix) {
+        while (of < G && pl.group_at[of + 1] == pl.group_at[of]) ++of;
+        if (of >= G) {
+          prefix = false;
+          of = 0;
+          at = suffix_at;
+          if (at >= stop) break;
+        }
+      }
+      if (!prefix)
+        while (of < B && pl.seq_at[of + 1] == pl.seq_at[of]) ++of;
+      of = __builtin_amdgcn_readfirstlane(of);
+      if (!prefix && of >= B) break;
+    }
+    idx = 0x7fffffff;
+    return false;
+  }
 };
 
 // LDS behind the plan, of shared items: two buffers of a tile, or, at a piece's
@@ -322,105 +432,152 @@ __host__ __device__ constexpr int end_bytes(int nr) {
 
 // The wave's rows: operand B of the key product, the keys each row sees, and
 // their softmax.
-template <int D, int NR>
+//
+// Softmax.  A row's probabilities are 2^(x - m) against a reference m, and its sum
+// and outputs in the same units.  m need not be the maximum: it only has to keep
+// the probabilities in range, and is moved, by the maximum of the tokens at hand,
+// when one of them reaches 2 -- seen by the exponent's top bit in the OR of
+// all of them, four instructions in place of the maximum's forty.  A move sets
+// m so that the largest probability is 2^-8 (f16 operands: 1, for their range), and
+// most rows move once.  The sum is one more row of the value product, of ones
+// (where the operand is the probability alone, without per-token value scales).
+template <int D, bool F16, bool PT, int NR>
 struct Rows {
+  static constexpr bool PF16 = F16 && !PT;  // f16 probabilities; with per-token scales bf16: a scale of any size times a
+                                            // probability stays in range
+  static constexpr float kHead = PF16 ? 0.0f : 8.0f;
   i32x4 q[NR][D / 32];
   f32x4 o[NR][D / 16];
-  float m[NR], l[NR];
+  f32x4 sum[NR];  // [0] (and, without per-token scales, all): of the row; with them the lane's part
+  float m[NR];
   int limit[NR];  // keys a row sees: below it
   int least;      // of all of the wave's
   float fac;      // of a raw logit, positive
+  int flip, keep; // bits of a query value to turn or keep: a negative scale's sign, a zero scale
 
-  // `wr`: which of the item's waves; DIMS16: a lane's k order is 16 dims of two
-  // steps (run_direct), else 8 of each.
-  template <bool DIMS16, bool PT>
-  __device__ __forceinline__ void load(const SpArgs& s, const Piece& pc, int wr, int c, int g) {
-    const pa_fp8_shared_prefix_args& a = s.a;
-    const int eq = s.eq, ql = a.query_length, gqa = a.query_group_size;
-    const float c0 = a.softmax_scale * kLog2e * (PT ? 1.0f : a.key_scale[0]);
+  __device__ __forceinline__ void set_scale(const SpArgs& s) {
+    const float c0 = s.a.softmax_scale * kLog2e * (PT ? 1.0f : s.a.key_scale[0]);
     fac = c0 == 0.0f ? 1.0f : fabsf(c0);
-    const int flip = c0 < 0.0f ? (int)0x80008000u : 0, keep = c0 == 0.0f ? 0 : -1;
-    least = 0x7fffffff;
+    flip = c0 < 0.0f ? (int)0x80008000u : 0;
+    keep = c0 == 0.0f ? 0 : -1;
+  }
+  // Row n's operand: 16-byte pieces k of the row, of 8 dims each.  DIMS16: a lane's
+  // k order is 16 dims of two steps (run_direct), else 8 of each.
+  template <bool DIMS16>
+  __device__ __forceinline__ void load_query(const SpArgs& s, const Piece& pc, int r, int g, i32x4 (&x)[D / 32]) const {
+    const pa_fp8_shared_prefix_args& a = s.a;
+    const bool live = r < pc.nrows;
+    const int bb = live ? r / s.eq : 0, e = live ? r - bb * s.eq : 0, qi = e / a.query_group_size;
+    const uint16_t* row = (const uint16_t*)a.query +
+                          ((int64_t)(pc.b0 + bb) * a.query_length + qi) * a.stride_q_tok +
+                          (int64_t)(pc.h * a.query_group_size + (e - qi * a.query_group_size)) * a.stride_q_head;
 #pragma unroll
-    for (int n = 0; n < NR; ++n) {
-      const int r = pc.row0 + (wr * NR + n) * 16 + c;
-      const bool live = r < pc.nrows;
-      const int bb = live ? r / eq : 0, e = live ? r - bb * eq : 0;
-      const int b = pc.b0 + bb, qi = e / gqa;
-      limit[n] = 0x7fffffff;
-      if (live) limit[n] = pa_min(pa_max(a.context_lengths[b] - ql + qi + 1, 0), pc.end);
-      least = pa_min(least, limit[n]);
-      const uint16_t* row = (const uint16_t*)a.query + (int64_t)(b * (int64_t)ql + qi) * a.stride_q_tok +
-                            (int64_t)(pc.h * gqa + (e - qi * gqa)) * a.stride_q_head;
+    for (int k = 0; k < D / 32; ++k) {
+      x[k] = i32x4{0, 0, 0, 0};
+      if (live) x[k] = *(const i32x4*)(row + (DIMS16 ? (4 * (k >> 1) + g) * 16 + 8 * (k & 1) : 32 * k + 8 * g));
+    }
+  }
+  // Row n begins, as row r of the piece's item, with operand x.
+  __device__ __forceinline__ void begin(const SpArgs& s, const Piece& pc, const int* ctx, int n, int r,
+                                        const i32x4 (&x)[D / 32]) {
+    const bool live = r < pc.nrows;
+    const int bb = live ? r / s.eq : 0, qi = live ? (r - bb * s.eq) / s.a.query_group_size : 0;
+    limit[n] = live ? pa_min(pa_max(ctx[pc.b0 + bb] - s.a.query_length + qi + 1, 0), pc.end) : 0x7fffffff;
+    if (n == 0 || limit[n] < least) least = limit[n];
+    if (n == NR - 1) {
 #pragma unroll
-      for (int k = 0; k < D / 32; ++k) {
-        i32x4 w = {0, 0, 0, 0};
-        if (live) w = *(const i32x4*)(row + (DIMS16 ? (4 * (k >> 1) + g) * 16 + 8 * (k & 1) : 32 * k + 8 * g));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = (w[i] ^ flip) & keep;
-        q[n][k] = w;
-      }
-      m[n] = kNegInf;
-      l[n] = 0.0f;
-#pragma unroll
-      for (int dt = 0; dt < D / 16; ++dt) o[n][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int d = 1; d < 16; d *= 2) least = pa_min(least, __shfl_xor(least, d, 64));
+      least = __builtin_amdgcn_readfirstlane(least);
     }
 #pragma unroll
-    for (int d = 1; d < 16; d *= 2) least = pa_min(least, __shfl_xor(least, d, 64));
-    least = __builtin_amdgcn_readfirstlane(least);
+    for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q[n][k][i] = (x[k][i] ^ flip) & keep;
+    m[n] = kNoKey;
+    sum[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) o[n][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // Moves the rows' references to where logits x (of the lane's row of each n)
-  // need them.
-  template <int NT>
-  __device__ __forceinline__ void reference(const f32x4 (&x)[NR][NT]) {
-    float top[NR];
-    bool moves = false;
+  // Probabilities of row n's logits of two key tiles.
+  __device__ __forceinline__ void exponentials(int n, const f32x4& x0, const f32x4& x1, float (&e)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(i < 4 ? x0[i] : x1[i - 4], fac, -m[n]));
+  }
+  static __device__ __forceinline__ i32x4 pack(const float (&e)[8]) {
+    return i32x4{round2<PF16>(e[0], e[1]), round2<PF16>(e[2], e[3]), round2<PF16>(e[4], e[5]), round2<PF16>(e[6], e[7])};
+  }
+
+  // The value product's operands for logits x0, x1 of every row.
+  __device__ __forceinline__ void weights(const f32x4 (&x0)[NR], const f32x4 (&x1)[NR], const f32x4& vs0, const f32x4& vs1,
+                                          i32x4 (&p)[NR]) {
+    float e[NR][8];
+    uint32_t high = 0;
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      top[n] = kNegInf;
+      exponentials(n, x0[n], x1[n], e[n]);
+      if constexpr (PT) {
 #pragma unroll
-      for (int T = 0; T < NT; ++T)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top[n] = fmaxf(top[n], x[n][T][i]);
-      top[n] = groups_max(top[n]) * fac;
-      moves |= top[n] > m[n] + kRescaleMargin;
+        for (int i = 0; i < 8; ++i) high |= __float_as_uint(e[n][i]);
+      } else {
+        p[n] = pack(e[n]);
+        high |= (uint32_t)(p[n][0] | p[n][1] | p[n][2] | p[n][3]);
+      }
     }
-    if (__ballot(moves)) {
+    if (__ballot((high & (PT ? 0x40000000u : 0x40004000u)) != 0)) {
+      move(x0, x1);
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
-        const float mn = top[n] > m[n] + kRescaleMargin ? top[n] : m[n];
-        const float f = mn == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m[n] - mn);
-        l[n] *= f;
+        exponentials(n, x0[n], x1[n], e[n]);
+        if constexpr (!PT) p[n] = pack(e[n]);
+      }
+    }
+    if constexpr (PT) {
 #pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) o[n][dt] *= f;
-        m[n] = mn;
+      for (int n = 0; n < NR; ++n) {
+        sum[n][0] += ((e[n][0] + e[n][1]) + (e[n][2] + e[n][3])) + ((e[n][4] + e[n][5]) + (e[n][6] + e[n][7]));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[n][i] *= i < 4 ? vs0[i] : vs1[i - 4];
+        p[n] = pack(e[n]);
       }
     }
   }
 
-  // Probabilities (times vs) of row n's logits of two key tiles, as an operand.
-  template <bool PT, bool PF16>
-  __device__ __forceinline__ i32x4 weights(int n, const f32x4& x0, const f32x4& x1, const f32x4& vs0, const f32x4& vs1) {
-    const float bias = m[n] == kNegInf ? 0.0f : -m[n];
-    float e[8], w[8];
+  // Moves the references of rows that x takes past them.
+  __device__ __forceinline__ void move(const f32x4 (&x0)[NR], const f32x4 (&x1)[NR]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(i < 4 ? x0[i] : x1[i - 4], fac, bias));
-      w[i] = PT ? e[i] * (i < 4 ? vs0[i] : vs1[i - 4]) : e[i];
+    for (int n = 0; n < NR; ++n) {
+      float top = kNegInf;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(fmaxf(x0[n][i], x1[n][i]), top);
+      top = groups_max(top) * fac;
+      const float to = top >= m[n] + 0.5f ? top + kHead : m[n];
+      const float f = __builtin_amdgcn_exp2f(m[n] - to);
+      m[n] = to;
+      sum[n] *= f;
+#pragma unroll
+      for (int dt = 0; dt < D / 16; ++dt) o[n][dt] *= f;
     }
-    l[n] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-    return i32x4{round2<PF16>(w[0], w[1]), round2<PF16>(w[2], w[3]), round2<PF16>(w[4], w[5]), round2<PF16>(w[6], w[7])};
   }
+  // The value product's row of ones.
+  __device__ __forceinline__ void add_sums(const i32x4 (&p)[NR]) {
+    if constexpr (!PT) {
+      constexpr int one = PF16 ? 0x3c003c00 : 0x3f803f80;
+#pragma unroll
+      for (int n = 0; n < NR; ++n) sum[n] = mfma<PF16>(i32x4{one, one, one, one}, p[n], sum[n]);
+    }
+  }
+  __device__ __forceinline__ float row_sum(int n) const { return PT ? groups_sum(sum[n][0]) : sum[n][0]; }
+  __device__ __forceinline__ float row_max(int n) const { return m[n] == kNoKey ? kNegInf : m[n]; }
 
   // Writes a piece that one wave worked alone.
   __device__ __forceinline__ void finish_alone(const Piece& pc, int c, int g) {
     static_assert(NR == 1, "one row tile");
-    l[0] = groups_sum(l[0]);
+    const float l = row_sum(0);
     if (pc.row0 + c >= pc.nrows) return;
     if (g == 0) {
-      pc.ml[c] = m[0];
-      pc.ml[pc.rows_out + c] = l[0];
+      pc.ml[c] = row_max(0);
+      pc.ml[pc.rows_out + c] = l;
     }
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) *(f32x4*)(pc.o + (int64_t)c * D + 16 * dt + 4 * g) = o[0][dt];
@@ -435,29 +592,29 @@ struct Rows {
     __syncthreads();                      // what LDS held before has been read
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      l[n] = groups_sum(l[n]);
+      const float l = row_sum(n);
       if (g == 0) {
-        lm[(wave * NR + n) * 16 + c] = m[n];
-        ll[(wave * NR + n) * 16 + c] = l[n];
+        lm[(wave * NR + n) * 16 + c] = row_max(n);
+        ll[(wave * NR + n) * 16 + c] = l;
       }
     }
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      float top = kNegInf, sum = 0.0f;
+      float top = kNegInf, all = 0.0f;
       for (int w = wr * wt; w < (wr + 1) * wt; ++w) top = fmaxf(top, lm[(w * NR + n) * 16 + c]);
       for (int w = wr * wt; w < (wr + 1) * wt; ++w) {
         const float mw = lm[(w * NR + n) * 16 + c];
         // (a wave that saw no key has 0 or, where its logits were NaN, NaN)
-        sum += ll[(w * NR + n) * 16 + c] * (mw == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mw - top));
+        all += ll[(w * NR + n) * 16 + c] * (mw == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mw - top));
       }
-      const float f = m[n] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m[n] - top);
+      const float f = m[n] == kNoKey ? 0.0f : __builtin_amdgcn_exp2f(m[n] - top);
 #pragma unroll
       for (int dt = 0; dt < D / 16; ++dt) o[n][dt] *= f;
       const int r = (wr * NR + n) * 16 + c;
       if (wi == 0 && g == 0 && pc.row0 + r < pc.nrows) {
         pc.ml[r] = top;
-        pc.ml[pc.rows_out + r] = sum;
+        pc.ml[pc.rows_out + r] = all;
       }
     }
     const int rows = SP_WAVES / wt * 16 * NR;
@@ -474,17 +631,19 @@ struct Rows {
         const int r = i >> 3, d = (i & 7) * 4;
         if (pc.row0 + r >= pc.nrows) break;  // (rows only grow with i)
         const int w0 = r / (16 * NR) * wt, rr = r % (16 * NR);
-        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-        for (int w = w0; w < w0 + wt; ++w) sum += *(const f32x4*)(lo + (w * 16 * NR + rr) * kOutStride + d);
-        *(f32x4*)(pc.o + (int64_t)r * D + 32 * d0 + d) = sum;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        for (int w = w0; w < w0 + wt; ++w) v += *(const f32x4*)(lo + (w * 16 * NR + rr) * kOutStride + d);
+        *(f32x4*)(pc.o + (int64_t)r * D + 32 * d0 + d) = v;
       }
     }
     __syncthreads();  // LDS is the next piece's
   }
 };
 
-// The item's pages: of a token, inside the cache and the table row whatever
-// the caller's table holds.
+// The item's pages: of a token (the same one in every lane), inside the cache and
+// the table row whatever the caller's table holds.  Scalar loads -- the launch
+// writes no table -- which wait by a counter of their own, so that the loads of
+// keys and values under way are not waited for.
 struct Pages {
   const int32_t* table;
   int last, lbs, blocks;
@@ -493,30 +652,21 @@ struct Pages {
         last(pa_min((pc.end - 1) >> s.lbs, s.a.max_blocks_per_seq - 1)),
         lbs(s.lbs),
         blocks(s.a.num_blocks) {}
-  __device__ __forceinline__ int operator()(int token) const {
-    int p = table[pa_min(token >> lbs, last)];
-    pa_note(p < 0 || p >= blocks, PA_VIOLATION_PAGE);
-    p = p < 0 ? 0 : p;
-    return p < blocks ? p : blocks - 1;
-  }
-};
-
-// The same for a token all lanes ask for: a scalar load (the launch writes no table).
-struct ScalarPages : Pages {
-  __device__ __forceinline__ ScalarPages(const SpArgs& s, const Piece& pc) : Pages(s, pc) {}
-  __device__ __forceinline__ int operator()(int token) const {
+  __device__ __forceinline__ int entry(int token) const {  // as it stands
     const int i = __builtin_amdgcn_readfirstlane(pa_min(token >> lbs, last));
-    int p = ((const __attribute__((address_space(4))) int32_t*)table)[i];
+    return ((const __attribute__((address_space(4))) int32_t*)table)[i];
+  }
+  __device__ __forceinline__ static int inside(int p, int blocks) {
     pa_note(p < 0 || p >= blocks, PA_VIOLATION_PAGE);
     p = p < 0 ? 0 : p;
     return p < blocks ? p : blocks - 1;
   }
+  __device__ __forceinline__ int operator()(int token) const { return inside(entry(token), blocks); }
 };
 
+// A piece worked by one wave.
 template <int D, bool F16, bool PT>
-__device__ __forceinline__ void run_direct(const SpArgs& s, const Piece& pc) {
-  // the value product of f16 queries with per-token scales runs in bf16: a
-  // scale of any size times a probability stays in range
+__device__ __forceinline__ void run_direct(const SpArgs& s, const Piece& pc, const int* ctx) {
   constexpr bool PF16 = F16 && !PT;
   const pa_fp8_shared_prefix_args& a = s.a;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
@@ -526,63 +676,83 @@ __device__ __forceinline__ void run_direct(const SpArgs& s, const Piece& pc) {
   const uint8_t* vbase = (const uint8_t*)a.value_cache + (int64_t)pc.h * a.stride_v_head;
   const int v_dim = a.trans_v ? 16 : bs, v_blk = a.trans_v ? D * 16 : 16;
   const int kblk = c >> 2;  // the lane's key tokens are of block kblk, its value tokens of block g
-  i32x4 kr[4][D / 64], vr[D / 16];
+  // Two tiles in flight (one beside per-token scales), in registers: a wave alone
+  // has no one else to wait with.
+  constexpr int kAhead = PT ? 1 : 2;
+  struct Tile {
+    i32x4 k[4][D / 64], v[D / 16];
+  };
+  Tile even, odd;
   f32x4 ks[4], vs[4];
-  auto load_keys = [&](int tile, int page) {
+  const int last = pc.tile_end - 1;
+  int entry[4];  // table entries of the tile to be loaded next, by token block
+  auto entries = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) entry[i] = page_of.entry(pa_min(tile, last) * SP_TILE + 16 * i);
+  };
+  auto page = [&](int blk) {  // of the lane's block
+    int p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = Pages::inside(entry[i], a.num_blocks);
+    return blk < 2 ? (blk == 0 ? p[0] : p[1]) : (blk == 2 ? p[2] : p[3]);
+  };
+  auto load_keys = [&](Tile& x, int tile) {
     const int in = ((tile * SP_TILE + 16 * kblk) & (bs - 1)) + (c & 3);
-    const uint8_t* p = kbase + (int64_t)page * a.stride_k_block + in * 16 + g * (bs * 16);
+    const uint8_t* p = kbase + (int64_t)page(kblk) * a.stride_k_block + in * 16 + g * (bs * 16);
 #pragma unroll
     for (int T = 0; T < 4; ++T)
 #pragma unroll
-      for (int u = 0; u < D / 64; ++u) kr[T][u] = *(const i32x4*)(p + 64 * T + (int64_t)(4 * u) * (bs * 16));
+      for (int u = 0; u < D / 64; ++u) x.k[T][u] = *(const i32x4*)(p + 64 * T + (int64_t)(4 * u) * (bs * 16));
   };
-  auto load_values = [&](int tile, int page) {
+  auto load_values = [&](Tile& x, int tile) {
     const int in = ((tile * SP_TILE + 16 * g) & (bs - 1)) >> 4;
-    const uint8_t* p = vbase + (int64_t)page * a.stride_v_block + in * v_blk + c * v_dim;
+    const uint8_t* p = vbase + (int64_t)page(g) * a.stride_v_block + in * v_blk + c * v_dim;
 #pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt) vr[dt] = *(const i32x4*)(p + (int64_t)(16 * dt) * v_dim);
+    for (int dt = 0; dt < D / 16; ++dt) x.v[dt] = *(const i32x4*)(p + (int64_t)(16 * dt) * v_dim);
   };
-  auto load_scales = [&](const float* base, int tile, int page, f32x4 (&x)[4]) {
-    const float* p = base + (int64_t)page * a.stride_ks_block + (int64_t)pc.h * a.stride_ks_head +
+  auto load_scales = [&](const float* base, int tile, f32x4 (&x)[4]) {
+    const float* p = base + (int64_t)page(g) * a.stride_ks_block + (int64_t)pc.h * a.stride_ks_head +
                      ((tile * SP_TILE + 16 * g) & (bs - 1));
 #pragma unroll
     for (int T = 0; T < 4; ++T) x[T] = *(const f32x4*)(p + 4 * T);
   };
 
-  int tile = pc.tile;
-  int kp = page_of(tile * SP_TILE + 16 * kblk), vp = page_of(tile * SP_TILE + 16 * g);
-  Rows<D, 1> w;
-  w.template load<true, PT>(s, pc, 0, c, g);
-  load_keys(tile, kp);
-  load_values(tile, vp);
+  Rows<D, F16, PT, 1> w;
+  w.set_scale(s);
+  entries(pc.tile);
+  i32x4 q[D / 32];
+  w.template load_query<true>(s, pc, pc.row0 + c, g, q);
+  load_keys(even, pc.tile);
+  load_values(even, pc.tile);
   if constexpr (PT) {
-    load_scales(a.key_scale, tile, vp, ks);
-    load_scales(a.value_scale, tile, vp, vs);
+    load_scales(a.key_scale, pc.tile, ks);
+    load_scales(a.value_scale, pc.tile, vs);
   }
-  {
-    const int next = pa_min(tile + 1, pc.tile_end - 1);
-    kp = page_of(next * SP_TILE + 16 * kblk);
-    vp = page_of(next * SP_TILE + 16 * g);
+  entries(pc.tile + 1);
+  if (kAhead == 2 && pc.tile < last) {
+    load_keys(odd, pc.tile + 1);
+    load_values(odd, pc.tile + 1);
+    entries(pc.tile + 2);
   }
-  for (; tile < pc.tile_end; ++tile) {
-    const int next = tile + 1;
-    const bool more = next < pc.tile_end;
-    f32x4 x[1][4];
+  w.begin(s, pc, ctx, 0, pc.row0 + c, q);
+  // tile from x, tile + kAhead into it
+  auto step = [&](Tile& x, int tile) {
+    const bool more = tile + kAhead <= last;
+    f32x4 l[4][1];
 #pragma unroll
     for (int T = 0; T < 4; ++T) {
-      x[0][T] = f32x4{0.f, 0.f, 0.f, 0.f};
+      l[T][0] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int u = 0; u < D / 64; ++u) {
-        const i32x4 k0 = widen8<F16>(kr[T][u][0], kr[T][u][1]), k1 = widen8<F16>(kr[T][u][2], kr[T][u][3]);
-        x[0][T] = mfma<F16>(k0, w.q[0][2 * u], x[0][T]);
-        x[0][T] = mfma<F16>(k1, w.q[0][2 * u + 1], x[0][T]);
+        l[T][0] = mfma<F16>(widen8<F16>(x.k[T][u][0], x.k[T][u][1]), w.q[0][2 * u], l[T][0]);
+        l[T][0] = mfma<F16>(widen8<F16>(x.k[T][u][2], x.k[T][u][3]), w.q[0][2 * u + 1], l[T][0]);
       }
     }
-    if (more) load_keys(next, kp);
+    if (more) load_keys(x, tile + kAhead);
     if constexpr (PT) {
 #pragma unroll
-      for (int T = 0; T < 4; ++T) x[0][T] *= ks[T];
-      if (more) load_scales(a.key_scale, next, vp, ks);
+      for (int T = 0; T < 4; ++T) l[T][0] *= ks[T];
+      if (more) load_scales(a.key_scale, tile + 1, ks);
     }
     // ---- masks: the part's first and last tiles ----
     const int t0 = tile * SP_TILE;
@@ -593,14 +763,14 @@ __device__ __forceinline__ void run_direct(const SpArgs& s, const Piece& pc) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int t = t0 + 16 * g + 4 * T + i;
-          if (t < pc.begin || t >= w.limit[0]) x[0][T][i] = kNegInf;
+          if (t < pc.begin || t >= w.limit[0]) l[T][0][i] = kNegInf;
         }
       // bytes behind the part's tokens may be anything, NaN among it
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int keep = (int)keep4(t0 + 16 * g + 4 * i, pc.begin, pc.end);
 #pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) vr[dt][i] &= keep;
+        for (int dt = 0; dt < D / 16; ++dt) x.v[dt][i] &= keep;
       }
       if constexpr (PT) {
 #pragma unroll
@@ -612,21 +782,26 @@ __device__ __forceinline__ void run_direct(const SpArgs& s, const Piece& pc) {
           }
       }
     }
-    w.reference(x);
-    const i32x4 p0 = w.template weights<PT, PF16>(0, x[0][0], x[0][1], vs[0], vs[1]);
-    const i32x4 p1 = w.template weights<PT, PF16>(0, x[0][2], x[0][3], vs[2], vs[3]);
+    i32x4 p[1];
+    w.weights(l[0], l[1], vs[0], vs[1], p);
+    w.add_sums(p);
 #pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt) {
-      const i32x4 v0 = widen8<PF16>(vr[dt][0], vr[dt][1]), v1 = widen8<PF16>(vr[dt][2], vr[dt][3]);
-      w.o[0][dt] = mfma<PF16>(v0, p0, w.o[0][dt]);
-      w.o[0][dt] = mfma<PF16>(v1, p1, w.o[0][dt]);
-    }
+    for (int dt = 0; dt < D / 16; ++dt) w.o[0][dt] = mfma<PF16>(widen8<PF16>(x.v[dt][0], x.v[dt][1]), p[0], w.o[0][dt]);
+    w.weights(l[2], l[3], vs[2], vs[3], p);
+    w.add_sums(p);
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) w.o[0][dt] = mfma<PF16>(widen8<PF16>(x.v[dt][2], x.v[dt][3]), p[0], w.o[0][dt]);
     if (more) {
-      load_values(next, vp);
-      if constexpr (PT) load_scales(a.value_scale, next, vp, vs);
-      const int after = pa_min(next + 1, pc.tile_end - 1);
-      kp = page_of(after * SP_TILE + 16 * kblk);
-      vp = page_of(after * SP_TILE + 16 * g);
+      load_values(x, tile + kAhead);
+      if constexpr (PT) load_scales(a.value_scale, tile + 1, vs);
+      entries(tile + kAhead + 1);
+    }
+  };
+  for (int tile = pc.tile; tile <= last; ++tile) {
+    step(even, tile);
+    if constexpr (kAhead == 2) {
+      if (++tile > last) break;
+      step(odd, tile);
     }
   }
   w.finish_alone(pc, c, g);
@@ -647,10 +822,10 @@ __host__ __device__ constexpr int work_bytes(int d, bool shared) {
 }
 
 // Masks of the scheduling groups.
-constexpr int kSchedAlu = 0x2, kSchedMfma = 0x8, kSchedDsRead = 0x100;
+constexpr int kSchedAlu = 0x2, kSchedMfma = 0x8, kSchedDsRead = 0x100, kSchedDsWrite = 0x200;
 
 template <int D, bool F16, bool PT, int NR, int WT>
-__device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, char* lds) {
+__device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, const int* ctx, char* lds) {
   constexpr bool PF16 = F16 && !PT;
   constexpr int NT = 4 / WT, NJ = 2 / WT;  // the wave's key tiles and value products
   constexpr int NS = D / 64;               // pieces of keys, and of values, that a thread brings
@@ -664,7 +839,7 @@ __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, cha
   // scalar but for a lane's constant offset.  Of the keys, lane (c, g) has token c
   // and dims 16 (g + 4 i) .. + 15; of the values, dims lane + 64 i; of the scales,
   // token c of the keys' (g = 0) or the values' (g = 1).
-  const ScalarPages page_of(s, pc);
+  const Pages page_of(s, pc);
   const uint8_t* kbase = (const uint8_t*)a.key_cache + (int64_t)pc.h * a.stride_k_head;
   const uint8_t* vbase = (const uint8_t*)a.value_cache + (int64_t)pc.h * a.stride_v_head;
   const int64_t s_head = (int64_t)pc.h * a.stride_ks_head;
@@ -688,9 +863,7 @@ __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, cha
       if (g < 2) sst = (g ? a.value_scale : a.key_scale)[at + c];
     }
   };
-  auto store = [&](int tile, int buffer) {
-    i32x4* lk = (i32x4*)(lds + buffer * tile_bytes(D));
-    i32x4* lv = lk + D / 8 * kKeyRow;
+  auto mask = [&](int tile) {
     const int t0 = tile * SP_TILE;
     if (t0 < pc.begin || t0 + SP_TILE > pc.end) {  // bytes outside the part may be anything, NaN among it
       asm volatile("");
@@ -705,6 +878,10 @@ __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, cha
         if (t < pc.begin || t >= pc.end) sst = 0.0f;
       }
     }
+  };
+  auto store = [&](int buffer) {
+    i32x4* lk = (i32x4*)(lds + buffer * tile_bytes(D));
+    i32x4* lv = lk + D / 8 * kKeyRow;
     const int row = (c >> 2) * kKeyTile + 4 * wave + (c & 3);  // row 4 wave + c % 4 of key tile c / 4
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
@@ -724,12 +901,20 @@ __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, cha
   };
 
   next_page(pc.tile);
-  Rows<D, NR> w;
-  w.template load<false, PT>(s, pc, wr, c, g);
+  Rows<D, F16, PT, NR> w;
+  w.set_scale(s);
+  {
+    i32x4 x[NR][D / 32];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) w.template load_query<false>(s, pc, pc.row0 + (wr * NR + n) * 16 + c, g, x[n]);
+#pragma unroll
+    for (int n = 0; n < NR; ++n) w.begin(s, pc, ctx, n, pc.row0 + (wr * NR + n) * 16 + c, x[n]);
+  }
   fetch(pc.tile);
   next_page(pa_min(pc.tile + 1, pc.tile_end - 1));
-  store(pc.tile, 0);
-  if (pc.tile + 1 < pc.tile_end) fetch(pc.tile + 1);
+  mask(pc.tile);
+  store(0);
+  fetch(pa_min(pc.tile + 1, pc.tile_end - 1));
   next_page(pa_min(pc.tile + 2, pc.tile_end - 1));
   __syncthreads();
   int buffer = 0;
@@ -740,8 +925,8 @@ __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, cha
     // Operand reads run a step ahead of the products, the first value product's
     // behind the keys' (left to itself, the compiler waits out the latency of
     // every read).
-    constexpr int K = D / 32, VA = D / 16, VP = VA / 2;
-    f32x4 x[NR][NT], vs[NT];
+    constexpr int K = D / 32, VA = D / 16, VP = D <= 128 ? VA / 2 : VA / 4;
+    f32x4 x[NT][NR], vs[2];
     i32x4 kf[K][NT], vf[VA];
     auto read_keys = [&](int k) {
 #pragma unroll
@@ -760,16 +945,15 @@ __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, cha
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int n = 0; n < NR; ++n) x[n][t] = mfma<F16>(kf[k][t], w.q[n][k], k ? x[n][t] : f32x4{0.f, 0.f, 0.f, 0.f});
+        for (int n = 0; n < NR; ++n) x[t][n] = mfma<F16>(kf[k][t], w.q[n][k], k ? x[t][n] : f32x4{0.f, 0.f, 0.f, 0.f});
     }
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (PT) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const f32x4 k4 = *(const f32x4*)(lsc + 16 * g + 4 * (wi * NT + t));
-        vs[t] = *(const f32x4*)(lsc + SP_TILE + 16 * g + 4 * (wi * NT + t));
 #pragma unroll
-        for (int n = 0; n < NR; ++n) x[n][t] *= k4;
+        for (int n = 0; n < NR; ++n) x[t][n] *= k4;
       }
     }
     const int t0 = tile * SP_TILE;
@@ -782,54 +966,60 @@ __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, cha
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int at = t0 + 16 * g + 4 * (wi * NT + t) + i;
-            if (at < pc.begin || at >= w.limit[n]) x[n][t][i] = kNegInf;
+            if (at < pc.begin || at >= w.limit[n]) x[t][n][i] = kNegInf;
           }
     }
-    w.reference(x);
     i32x4 p[NR];
-#pragma unroll
-    for (int n = 0; n < NR; ++n) p[n] = w.template weights<PT, PF16>(n, x[n][0], x[n][1], vs[0], vs[1]);
-    // the first product beside the second half's probabilities, reads VP ahead
-    __builtin_amdgcn_sched_barrier(0);
-    i32x4 p1[NR], vf1[VA];
+    auto value_scales = [&](int t) {
+      if constexpr (PT) {
+        vs[0] = *(const f32x4*)(lsc + SP_TILE + 16 * g + 4 * (wi * NT + t));
+        vs[1] = *(const f32x4*)(lsc + SP_TILE + 16 * g + 4 * (wi * NT + t + 1));
+      }
+    };
+    value_scales(0);
+    w.weights(x[0], x[1], vs[0], vs[1], p);
     if constexpr (NJ == 2) {
-#pragma unroll
-      for (int n = 0; n < NR; ++n) p1[n] = w.template weights<PT, PF16>(n, x[n][2], x[n][3], vs[2], vs[3]);
-    }
-#pragma unroll
-    for (int i = VP; i < VP + VA; ++i) {
-      if (i < VA)
-        vf[i] = lv[(2 * g + wi * NJ) * D + 16 * i + c];
-      else if (NJ == 2)
-        vf1[i - VA] = lv[(2 * g + 1) * D + 16 * (i - VA) + c];
-#pragma unroll
-      for (int n = 0; n < NR; ++n) w.o[n][i - VP] = mfma<PF16>(vf[i - VP], p[n], w.o[n][i - VP]);
-    }
-#pragma unroll
-    for (int dt = 0; dt < VA; ++dt) {
-      __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(kSchedMfma, NR, 0);
-      if (NJ == 2) __builtin_amdgcn_sched_group_barrier(kSchedAlu, (PT ? 40 : 32) * NR * 16 / D, 0);
-    }
-    if constexpr (NJ == 2) {
+      // the first product beside the second half's probabilities, reads VP ahead
       __builtin_amdgcn_sched_barrier(0);
+      w.add_sums(p);
 #pragma unroll
       for (int i = VP; i < VP + VA; ++i) {
-        if (i < VA) vf1[i] = lv[(2 * g + 1) * D + 16 * i + c];
+        if (i < VA) vf[i] = lv[2 * g * D + 16 * i + c];
 #pragma unroll
-        for (int n = 0; n < NR; ++n) w.o[n][i - VP] = mfma<PF16>(vf1[i - VP], p1[n], w.o[n][i - VP]);
+        for (int n = 0; n < NR; ++n) w.o[n][i - VP] = mfma<PF16>(vf[i - VP], p[n], w.o[n][i - VP]);
       }
+#pragma unroll
+      for (int dt = 0; dt < VP; ++dt) vf[dt] = lv[(2 * g + 1) * D + 16 * dt + c];
 #pragma unroll
       for (int dt = 0; dt < VA; ++dt) {
         __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 1, 0);
         __builtin_amdgcn_sched_group_barrier(kSchedMfma, NR, 0);
+        __builtin_amdgcn_sched_group_barrier(kSchedAlu, NR * 24 / VA, 0);
       }
+      value_scales(2);
+      w.weights(x[2], x[3], vs[0], vs[1], p);
     }
-    if (tile + 1 < pc.tile_end) {
-      store(tile + 1, buffer ^ 1);
-      if (tile + 2 < pc.tile_end) fetch(tile + 2);
-      next_page(pa_min(tile + 3, pc.tile_end - 1));
+    // the last product beside the next tile's way into LDS (behind the last tile:
+    // once more the last, which no one reads)
+    mask(pa_min(tile + 1, pc.tile_end - 1));
+    __builtin_amdgcn_sched_barrier(0);
+    w.add_sums(p);
+#pragma unroll
+    for (int i = VP; i < VP + VA; ++i) {
+      if (i < VA) vf[i] = lv[(2 * g + wi * NJ + NJ - 1) * D + 16 * i + c];
+#pragma unroll
+      for (int n = 0; n < NR; ++n) w.o[n][i - VP] = mfma<PF16>(vf[i - VP], p[n], w.o[n][i - VP]);
     }
+    store(buffer ^ 1);
+#pragma unroll
+    for (int dt = 0; dt < VA; ++dt) {
+      if (dt < VA - VP) __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kSchedMfma, NR, 0);
+      __builtin_amdgcn_sched_group_barrier(kSchedAlu, 4, 0);
+      __builtin_amdgcn_sched_group_barrier(kSchedDsWrite, 1, 0);
+    }
+    fetch(pa_min(tile + 2, pc.tile_end - 1));
+    next_page(pa_min(tile + 3, pc.tile_end - 1));
     __syncthreads();
   }
   w.finish(pc, lds, WT, wave, wr, wi, c, g);
@@ -841,100 +1031,14 @@ static_assert(end_bytes(2) <= 2 * tile_bytes(64), "a piece's end fits the tiles'
 // The kernels
 // ---------------------------------------------------------------------------
 
-// Works the tiles of the line's region [from, to) that begin in [lo, hi) (the
-// share of `worker`, as long as `share`): a workgroup's (WAVE false) or a wave's.
-template <int D, bool F16, bool PT, bool WAVE>
-__device__ __forceinline__ void walk(const SpArgs& s, const Plan& pl, int64_t prefix_line, int64_t from, int64_t to,
-                                     int64_t lo, int64_t hi, int64_t share, int worker, char* work) {
-  const int B = s.a.num_seqs, G = s.a.num_groups, H = s.a.num_kv_heads;
-  const int64_t start = lo > from ? lo : from, stop = hi < to ? hi : to;
-  if (start >= stop) return;
-  // The item that holds position `start`, then those behind it: `of` a group or a
-  // sequence, `idx` the item among its own (kv head outer, row tile inner).
-  bool prefix = start < prefix_line;
-  int of = __builtin_amdgcn_readfirstlane(prefix ? last_le(pl.group_at, G, start, H)
-                                                 : last_le(pl.seq_at, B, start - prefix_line, H));
-  int idx = -1;
-  int64_t at = 0;  // of item idx
-  while (true) {
-    const SpShape& sh = prefix ? s.p : s.s;
-    int begin, end, tiles;
-    if (prefix) {
-      tiles = pl.row_tiles[of + 1] - pl.row_tiles[of];
-      begin = 0;
-      end = pl.len[of];
-    } else {
-      const int gr = group_of(pl, G, of);
-      tiles = s.col_tiles;
-      begin = gr >= 0 ? pl.len[gr] : 0;
-      end = pl.ctx[of];
-    }
-    tiles = __builtin_amdgcn_readfirstlane(tiles);
-    begin = __builtin_amdgcn_readfirstlane(begin);
-    end = __builtin_amdgcn_readfirstlane(end);
-    const int n = sp_tiles(begin, end), cost = sp_item_cost(sh, n);
-    if (idx < 0) {  // the first one
-      const int64_t of_at = prefix ? (int64_t)H * pl.group_at[of] : prefix_line + (int64_t)H * pl.seq_at[of];
-      idx = __builtin_amdgcn_readfirstlane(sp_worker_of(start - of_at, cost));
-      at = of_at + (int64_t)idx * cost;
-    }
-    for (; idx < H * tiles && at < stop; ++idx, at += cost) {
-      const int t0 = __builtin_amdgcn_readfirstlane(sp_tile_from(sh, lo, at, n));
-      const int t1 = __builtin_amdgcn_readfirstlane(sp_tile_from(sh, hi, at, n));
-      if (t1 <= t0) continue;
-      const int item = __builtin_amdgcn_readfirstlane(prefix ? H * pl.row_tiles[of] + idx : of * H * tiles + idx);
-      const int h = idx / tiles, slot = item + worker;
-      Piece pc;
-      pc.b0 = prefix ? __builtin_amdgcn_readfirstlane(pl.first[of]) : of;
-      pc.h = h;
-      pc.row0 = (idx - h * tiles) * sh.rows;
-      pc.nrows = prefix ? __builtin_amdgcn_readfirstlane((pl.first[of + 1] - pl.first[of]) * s.eq) : s.eq;
-      pc.begin = begin;
-      pc.end = end;
-      pc.tile = begin / SP_TILE + t0;
-      pc.tile_end = begin / SP_TILE + t1;
-      pc.rows_out = prefix ? s.p_rows : s.s_rows;
-      pc.ml = (prefix ? s.p_ml : s.s_ml) + (int64_t)slot * 2 * pc.rows_out;
-      pc.o = (prefix ? s.p_o : s.s_o) + (int64_t)slot * pc.rows_out * D;
-      if (t0 == 0 && (WAVE ? (threadIdx.x & 63) : threadIdx.x) == 0) {
-        const int last = sp_worker_of(at + sh.overhead + (int64_t)(n - 1) * sh.cost, share);
-        s.items[prefix ? item : s.max_prefix_items + item] = int2{slot, last - worker + 1};
-      }
-      if constexpr (WAVE) {
-        run_direct<D, F16, PT>(s, pc);
-      } else {
-        constexpr int most = D <= 128 ? 2 : 1;
-        if (sh.wt == 1)
-          run_shared<D, F16, PT, most, 1>(s, pc, work);
-        else if (most == 1 || sh.nr == 1)
-          run_shared<D, F16, PT, 1, 2>(s, pc, work);
-        else
-          run_shared<D, F16, PT, most, 2>(s, pc, work);
-      }
-    }
-    if (at >= stop) return;
-    // on to the next group or sequence that has items
-    idx = 0;
-    ++of;
-    if (prefix) {
-      while (of < G && pl.group_at[of + 1] == pl.group_at[of]) ++of;
-      if (of >= G) {
-        prefix = false;
-        of = 0;
-      }
-    }
-    if (!prefix)
-      while (of < B && pl.seq_at[of + 1] == pl.seq_at[of]) ++of;
-    if (!prefix && of >= B) return;
-    of = __builtin_amdgcn_readfirstlane(of);
-  }
-}
-
 template <int D, bool F16, bool PT>
 __global__ __launch_bounds__(kThreads, 2) void pa_shared_prefix_kernel(const SpArgs s) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const pa_fp8_shared_prefix_args& a = s.a;
   const int B = a.num_seqs, G = a.num_groups, H = a.num_kv_heads;
+  // every line of the arguments is asked for at once, not one by one where first used
+  asm volatile("" ::"s"(a.context_lengths), "s"(a.stride_k_block), "s"(a.stride_out_tok), "s"(a.block_size), "s"(s.p.rows),
+               "s"(s.s.overhead), "s"(s.seq_info), "s"(s.p_o), "s"(s.s_o));
   const Plan pl = plan_of(lds, B, G);
   char* const work = lds + plan_bytes(B, G);
   make_plan(pl, s);
@@ -952,85 +1056,119 @@ __global__ __launch_bounds__(kThreads, 2) void pa_shared_prefix_kernel(const SpA
     s.seq_info[b] = v;
   }
 
-  const int64_t prefix_line = (int64_t)H * pl.group_at[G], line = prefix_line + (int64_t)H * pl.seq_at[B];
-  const int64_t share = sp_share(line, gridDim.x);
-  const int64_t lo = (int64_t)worker * share;
+  // the line: prefix items from 0, suffix items from `suffix_at`; the shared ones
+  // first (prefix items have at least a suffix item's rows)
+  const int64_t prefix_cost = (int64_t)H * pl.group_at[G], suffix_cost = (int64_t)H * pl.seq_at[B];
+  const int64_t shared = (s.p.shared ? prefix_cost : 0) + (s.s.shared ? suffix_cost : 0);
+  const int64_t share = sp_share(shared, prefix_cost + suffix_cost - shared, gridDim.x);
+  const int64_t direct_at = sp_direct_at(shared, share, gridDim.x);
+  const int64_t suffix_at = s.s.shared || !s.p.shared ? prefix_cost : direct_at;
+  const int64_t line = suffix_at + suffix_cost, lo = (int64_t)worker * share;
   if (lo >= line) return;
-  // shared items first, the workgroup together (prefix items have at least a
-  // suffix item's rows, so direct prefix items mean direct suffix items)
-  const int64_t shared_line = s.s.shared ? line : (s.p.shared ? prefix_line : 0);
-  walk<D, F16, PT, false>(s, pl, prefix_line, 0, shared_line, lo, lo + share, share, worker, work);
+  Walk walk;
+  walk.start(s, pl, suffix_at, 0, shared, lo, share, worker);
+  Piece pc;
+  while (walk.next_piece(s, pl, D, false, pc)) {
+    const SpShape& sh = pc.of_prefix ? s.p : s.s;
+    constexpr int most = D <= 128 ? 2 : 1;
+    if (sh.wt == 1)
+      run_shared<D, F16, PT, most, 1>(s, pc, pl.ctx, work);
+    else if (most == 1 || sh.nr == 1)
+      run_shared<D, F16, PT, 1, 2>(s, pc, pl.ctx, work);
+    else
+      run_shared<D, F16, PT, most, 2>(s, pc, pl.ctx, work);
+  }
   if constexpr (D <= 128) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t quarter = share / SP_WAVES, wlo = lo + wave * quarter;
-    walk<D, F16, PT, true>(s, pl, prefix_line, shared_line, line, wlo, wlo + quarter, quarter, worker * SP_WAVES + wave,
-                           nullptr);
+    const int64_t quarter = share / SP_WAVES;
+    walk.start(s, pl, suffix_at, direct_at, line, lo + wave * quarter, quarter, worker * SP_WAVES + wave);
+    while (walk.next_piece(s, pl, D, true, pc)) run_direct<D, F16, PT>(s, pc, pl.ctx);
   }
 }
 
 constexpr int kMergeThreads = 256;
 
 // out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over a row's pieces.
-// Workgroup (sequence and kv head, block of columns): D / 4 threads hold a
-// row's four dims each; where the block has fewer columns than the workgroup
-// has such teams, several teams share a row's pieces and meet in LDS.
+// Workgroup (sequence and kv head, block of columns): D / 4 threads, a team,
+// hold a row's four dims each; `shares` teams (a power of two) share a row's
+// pieces, four of them in flight each, and meet in LDS.
 template <int D, bool PT>
-__global__ __launch_bounds__(kMergeThreads) void pa_shared_prefix_merge_kernel(const SpArgs s, int block_cols) {
+__global__ __launch_bounds__(kMergeThreads) void pa_shared_prefix_merge_kernel(const SpArgs s, int shares) {
   constexpr int kTeam = D / 4, kTeams = kMergeThreads / kTeam;
   __shared__ float lm[kTeams], ll[kTeams];
   __shared__ __attribute__((aligned(16))) f32x4 lo[kMergeThreads];
   const pa_fp8_shared_prefix_args& a = s.a;
   const int H = a.num_kv_heads, b = blockIdx.x / H, h = blockIdx.x - b * H;
   const int team = threadIdx.x / kTeam, d = (threadIdx.x - team * kTeam) * 4;
-  const int shares = kTeams / block_cols;  // teams a column
+  const int block_cols = kTeams / shares;
   const int col = team / shares, share = team - col * shares;
   const int e = blockIdx.y * block_cols + col;
-  const bool live = team < shares * block_cols && e < s.eq;
+  const bool live = col < block_cols && e < s.eq;
 
+  asm volatile("" ::"s"(a.value_scale), "s"(a.stride_out_head), "s"(a.output_dtype), "s"(s.p.rows), "s"(s.items), "s"(s.p_o),
+               "s"(s.s_o));  // (as above)
   const int4 info = s.seq_info[b];
-  float m = kNegInf, l = 0.0f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  auto take = [&](const float* ml, const float* po, int rows, int slot, int pieces, int r) {
-    for (int i = share; i < pieces; i += shares) {
-      const int64_t at = slot + i;
-      const float mi = ml[at * 2 * rows + r], li = ml[at * 2 * rows + rows + r];
-      const f32x4 oi = *(const f32x4*)(po + (at * rows + r) * D + d);
-      const float mn = fmaxf(m, mi);
-      const float f = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-      const float fi = mi == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mi - mn);
-      l = l * f + li * fi;
-      o = o * f + oi * fi;
-      m = mn;
-    }
-  };
+  // the row's pieces: n[0] in the prefix's slots, n[1] in the suffix's
+  int first[2] = {0, 0}, n[2] = {0, 0}, row[2] = {0, 0};
   if (live) {
     if (info.x >= 0) {
-      const int row = info.y + e, t = row / s.p.rows;
+      const int r = info.y + e, t = r / s.p.rows;
       const int2 it = s.items[info.x + h * info.z + t];
-      take(s.p_ml, s.p_o, s.p_rows, it.x, it.y, row - t * s.p.rows);
+      first[0] = it.x;
+      n[0] = it.y;
+      row[0] = r - t * s.p.rows;
     }
     if (info.w) {
       const int t = e / s.s.rows;
       const int2 it = s.items[s.max_prefix_items + (b * H + h) * s.col_tiles + t];
-      take(s.s_ml, s.s_o, s.s_rows, it.x, it.y, e - t * s.s.rows);
+      first[1] = it.x;
+      n[1] = it.y;
+      row[1] = e - t * s.s.rows;
     }
   }
+  float m = kNegInf, l = 0.0f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  auto add = [&](float mi, float li, const f32x4& oi) {
+    const float mn = fmaxf(m, mi);
+    const float f = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+    const float fi = mi == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mi - mn);
+    l = l * f + li * fi;
+    o = o * f + oi * fi;
+    m = mn;
+  };
+  constexpr int kAhead = 4;
+  for (int i0 = share; i0 < n[0] + n[1]; i0 += kAhead * shares) {
+    float mi[kAhead], li[kAhead];
+    f32x4 oi[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = i0 + k * shares;
+      const bool in = i < n[0] + n[1], p = i < n[0];
+      const int rows = p ? s.p_rows : s.s_rows, r = p ? row[0] : row[1];
+      const int64_t slot = in ? (p ? first[0] + i : first[1] + i - n[0]) : 0;
+      const float* ml = (p || !in ? s.p_ml : s.s_ml) + slot * 2 * rows + r;
+      const float* po = (p || !in ? s.p_o : s.s_o) + (slot * rows + r) * D + d;
+      mi[k] = kNegInf;
+      li[k] = 0.0f;
+      oi[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (in) {
+        mi[k] = ml[0];
+        li[k] = ml[rows];
+        oi[k] = *(const f32x4*)po;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) add(mi[k], li[k], oi[k]);
+  }
   if (shares > 1) {
-    if (d == 0) {
+    if (d == 0 && team < kTeams) {
       lm[team] = m;
       ll[team] = l;
     }
     lo[threadIdx.x] = o;
     __syncthreads();
     if (!live || share) return;
-    for (int i = 1; i < shares; ++i) {
-      const float mi = lm[team + i], mn = fmaxf(m, mi);
-      const float f = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-      const float fi = mi == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mi - mn);
-      l = l * f + ll[team + i] * fi;
-      o = o * f + lo[threadIdx.x + i * kTeam] * fi;
-      m = mn;
-    }
+    for (int i = 1; i < shares; ++i) add(lm[team + i], ll[team + i], lo[threadIdx.x + i * kTeam]);
   }
   if (!live) return;
   // a row that sees no key is zero
@@ -1100,13 +1238,15 @@ hipError_t launch(const SpArgs& s, hipStream_t st) {
   hipLaunchKernelGGL((pa_shared_prefix_kernel<D, F16, PT>), dim3(s.a.num_workers), dim3(kThreads), lds, st, s);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  constexpr int teams = kMergeThreads / (D / 4);
-  int cols = 1;
-  while (cols < teams && cols < s.eq) cols *= 2;
-  if (cols > teams) cols = teams;
+  // Teams of a row: about a quarter of the pieces that the workers leave of an
+  // item at most, and no fewer than the columns leave idle.
+  constexpr int teams = 1 << (31 - __builtin_clz(kMergeThreads / (D / 4)));
+  const int pieces = s.a.num_workers / pa_max(1, s.prefix_items);
+  int shares = 1;
+  while (shares < teams && (shares * s.eq < teams || shares * 4 < pieces)) shares *= 2;
   hipLaunchKernelGGL((pa_shared_prefix_merge_kernel<D, PT>),
-                     dim3((unsigned)(s.a.num_seqs * s.a.num_kv_heads), (unsigned)pa_cdiv(s.eq, cols)),
-                     dim3(kMergeThreads), 0, st, s, cols);
+                     dim3((unsigned)(s.a.num_seqs * s.a.num_kv_heads), (unsigned)pa_cdiv(s.eq, kMergeThreads / (D / 4) / shares)),
+                     dim3(kMergeThreads), 0, st, s, shares);
   return hipGetLastError();
 }
 
@@ -1147,7 +1287,6 @@ extern "C" int pa_fp8_plan_shared_prefix(const int32_t* context_lengths, const i
     int of, h0, items, begin, tiles, base;
   };
   std::vector<Kind> line;
-  int64_t total = 0;
   for (int g = 0; g < G; ++g) {
     const int rows = (first[g + 1] - first[g]) * z.eq;
     len[g] = rows > 0 ? pa_min(pa_max(prefix_lengths[g], 0), capacity) : 0;
@@ -1155,24 +1294,30 @@ extern "C" int pa_fp8_plan_shared_prefix(const int32_t* context_lengths, const i
     tiles[g + 1] = tiles[g] + (len[g] > 0 ? pa_cdiv(rows, z.p.rows) : 0);
     const int n = tiles[g + 1] - tiles[g], steps = sp_tiles(0, len[g]);
     if (n > 0) line.push_back({true, g, n, H * n, 0, steps, H * tiles[g]});
-    total += (int64_t)H * n * sp_item_cost(z.p, steps);
   }
   for (int b = 0; b < B; ++b) {
     const int end = pa_min(pa_max(context_lengths[b], 0), capacity);
     const int steps = sp_tiles(seq_len[b], end);
     if (steps > 0) line.push_back({false, b, z.col_tiles, H * z.col_tiles, seq_len[b], steps, b * H * z.col_tiles});
-    total += (int64_t)H * z.col_tiles * sp_item_cost(z.s, steps);
   }
-  if (total == 0) return 0;
-  const int64_t share = sp_share(total, workers);
+  int64_t cost[2] = {0, 0};  // of the suffix and the prefix items
+  for (const Kind& k : line) cost[k.prefix] += (int64_t)k.items * sp_item_cost(k.prefix ? z.p : z.s, k.tiles);
+  const int64_t shared = (z.p.shared ? cost[1] : 0) + (z.s.shared ? cost[0] : 0);
+  const int64_t share = sp_share(shared, cost[0] + cost[1] - shared, workers);
+  const int64_t suffix_at = z.s.shared || !z.p.shared ? cost[1] : sp_direct_at(shared, share, workers);
   int n = 0;
   int64_t at = 0;
+  bool prefix = true;
   for (const Kind& k : line) {
+    if (prefix && !k.prefix) {
+      prefix = false;
+      at = suffix_at;
+    }
     const SpShape& sh = k.prefix ? z.p : z.s;
     const int64_t q = sh.shared ? share : share / SP_WAVES;
     for (int i = 0; i < k.items; ++i) {
       const int w0 = sp_worker_of(at + sh.overhead, q);
-      const int w1 = sp_worker_of(at + sh.overhead + (int64_t)(k.tiles - 1) * sh.cost, q);
+      const int w1 = sp_worker_of(at + sh.overhead + ((int64_t)(k.tiles - 1) << sh.lcost), q);
       for (int w = w0; w <= w1; ++w) {
         const int t0 = k.begin / SP_TILE + sp_tile_from(sh, w * q, at, k.tiles);
         const int t1 = k.begin / SP_TILE + sp_tile_from(sh, (w + 1) * q, at, k.tiles);
@@ -1229,6 +1374,7 @@ extern "C" int pa_fp8_decode_shared_prefix(const pa_fp8_shared_prefix_args* a, v
   s.seq_info = (int4*)(ws + z.seq_info);
   s.items = (int2*)(ws + z.items);
   s.max_prefix_items = (int)z.prefix_items;
+  s.prefix_items = a->num_groups > 0 ? (int)((int64_t)z.eq * a->num_seqs / z.p.rows + 1) * a->num_kv_heads : 1 << 20;
   s.p_ml = (float*)(ws + z.p_ml);
   s.p_o = (float*)(ws + z.p_o);
   s.s_ml = (float*)(ws + z.s_ml);

@@ -26,14 +26,14 @@
 #define SP_MAX_SEQS 4096    // the plan of a launch is held in LDS
 #define SP_MAX_GROUPS 1024
 #define SP_MAX_TOKENS (1 << 30)  // of a table row: larger ones count as this
-#define SP_MIN_SHARE 120         // at least a shared tile, and four of a wave's pieces
+#define SP_MIN_SHARE 160         // at least a shared tile, and four of a wave's pieces
 
 typedef struct SpShape {
   int shared;    // tiles come through LDS to a workgroup; else a wave works alone
   int nr;        // 16-row tiles of a wave
   int wt;        // waves that hold the same rows (shared)
   int rows;      // of an item
-  int cost;      // of a tile, in eighths of a microsecond of one wave
+  int lcost;     // log2 of a tile's cost, in eighths of a microsecond of one wave
   int overhead;  // of beginning and ending a piece
 } SpShape;
 
@@ -48,22 +48,25 @@ PA_HD SpShape sp_shape(int rows, int head_size) {
   s.nr = rows > 32 ? most : 1;
   s.wt = !s.shared ? 1 : (rows > 32 * s.nr ? 1 : 2);
   s.rows = s.shared ? 16 * s.nr * (SP_WAVES / s.wt) : 16;
-  s.cost = s.shared ? (s.wt == 1 ? 60 : 42) : 8;
-  s.overhead = s.shared ? 120 : 24;
+  s.lcost = s.shared ? 6 : 4;
+  s.overhead = s.shared ? 160 : 40;
   return s;
 }
 
 PA_HD int sp_tiles(int first_token, int end_token) {
   return end_token <= first_token ? 0 : pa_cdiv(end_token, SP_TILE) - first_token / SP_TILE;
 }
-PA_HD int sp_item_cost(const SpShape& s, int tiles) { return tiles > 0 ? s.overhead + tiles * s.cost : 0; }
+PA_HD int sp_item_cost(const SpShape& s, int tiles) { return tiles > 0 ? s.overhead + (tiles << s.lcost) : 0; }
 
-// A workgroup's share of the line: a multiple of four that no worker's part of
-// is shorter than a tile.
-PA_HD int64_t sp_share(int64_t line, int workers) {
+// A workgroup's share of a line of shared and direct items: a multiple of four that
+// no worker's part of is shorter than a tile.  The direct items begin with a
+// workgroup of their own (sp_direct_at): a wave's quarter of a share takes as long
+// as a workgroup's whole one, so a workgroup with both would take twice as long.
+PA_HD int64_t sp_share(int64_t shared, int64_t direct, int workers) {
+  const int w = shared > 0 && direct > 0 && workers > 1 ? workers - 1 : workers;
+  const int64_t line = shared + direct;
   // (the usual line needs no 64-bit division)
-  int64_t q = line < 0x40000000 ? (int64_t)(((uint32_t)line + workers - 1) / (uint32_t)workers)
-                                : (line + workers - 1) / workers;
+  int64_t q = line < 0x40000000 ? (int64_t)(((uint32_t)line + w - 1) / (uint32_t)w) : (line + w - 1) / w;
   q = (q + 3) & ~(int64_t)3;
   return q < SP_MIN_SHARE ? SP_MIN_SHARE : q;
 }
@@ -71,10 +74,14 @@ PA_HD int64_t sp_share(int64_t line, int workers) {
 PA_HD int sp_worker_of(int64_t x, int64_t share) {
   return x < 0x40000000 && share < 0x40000000 ? (int)((uint32_t)x / (uint32_t)share) : (int)(x / share);
 }
+// Where the direct items begin on the line.
+PA_HD int64_t sp_direct_at(int64_t shared, int64_t share, int workers) {
+  return workers > 1 && shared > 0 ? (int64_t)(sp_worker_of(shared - 1, share) + 1) * share : shared;
+}
 // First tile of an item at position `at` that begins at or behind x.
 PA_HD int sp_tile_from(const SpShape& s, int64_t x, int64_t at, int tiles) {
   const int64_t d = x - at - s.overhead;
   if (d <= 0) return 0;
-  if (d > (int64_t)tiles * s.cost) return tiles;
-  return (int)(((uint32_t)d + s.cost - 1) / (uint32_t)s.cost);  // (a row's tiles times their cost: below 2^31)
+  if (d > (int64_t)tiles << s.lcost) return tiles;
+  return (int)(((uint32_t)d + (1u << s.lcost) - 1) >> s.lcost);  // (a row's tiles times their cost: below 2^31)
 }

@@ -4,7 +4,8 @@ The bound of an output (derived, nothing fitted).  With u_p the half step of
 the probabilities' type (bf16 2^-8; f16 2^-11, where half-precision queries
 meet per-tensor scales), u_o that of the output's, a = sum p |v| and dx the
 size of a row's largest logit sum:
-  * rounding the probabilities moves the output by at most u_p a (f16's
+  * rounding the probabilities moves the output by at most u_p a, and, where the
+    sum is that of the rounded ones (per-tensor scales), by u_p |out| more (f16's
     subnormals by a further 2^-25 max|v| a token: the reference exponent keeps
     the largest sum at 1 or more);
   * a logit is a float32 sum of D products and a few float32 factors: it is
@@ -51,7 +52,7 @@ def check(d, out, ref=None):
     f16 = d["query"].dtype == torch.float16 and d["key_scale"].dim() == 1
     u_p = U[torch.float16] if f16 else U[torch.bfloat16]
     e = (D + 8) * 2.0**-24 * dx + 2.0**-21
-    tol = (u_p + 2 * e + 2 * (n + 64) * 2.0**-24) * a + U[out.dtype] * want.abs() + 1e-30
+    tol = (u_p + 2 * e + 2 * (n + 64) * 2.0**-24) * a + (U[out.dtype] + u_p) * want.abs() + 1e-30
     if f16:
         tol = tol + n * 2.0**-25 * 448 * d["value_scale"].double().max()
     err = (out.double() - want).abs()
