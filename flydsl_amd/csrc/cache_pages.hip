@@ -375,70 +375,104 @@ struct Extend {
   int32_t* src;    // shared partial page to copy, or -1
 };
 
+// For each entry i of list[0 .. n) (LDS): how many entries before it are equal to
+// it (and not negative).  The threads of an entry share the entries before it, so
+// that a short list takes few turns; out[] is cleared and complete on return.
+__device__ __forceinline__ void count_before(const int* list, int n, int* out) {
+  for (int i = threadIdx.x; i < n; i += kPlanThreads) out[i] = 0;
+  __syncthreads();
+  int wide = 64;  // entries at a time: whole waves, whose reads are broadcasts
+  while (wide < n && wide < kPlanThreads) wide *= 2;
+  const int parts = kPlanThreads / wide, part = (int)threadIdx.x / wide;
+  for (int i = (int)threadIdx.x % wide; i < n; i += wide) {
+    const int v = list[i];
+    if (v < 0) continue;
+    const int4* at = reinterpret_cast<const int4*>(list);
+    int count = 0;
+#pragma unroll 4
+    for (int j = part; 4 * j < i; j += parts) {
+      const int4 w = at[j];
+      count += (w.x == v) + (w.y == v && 4 * j + 1 < i) + (w.z == v && 4 * j + 2 < i) +
+               (w.w == v && 4 * j + 3 < i);
+    }
+    if (count) atomicAdd(&out[i], count);
+  }
+  __syncthreads();
+}
+
 // Workgroups 0 .. chunks - 1 count the pool, the last one plans the
 // sequences: what each needs, and where in the row of given pages it begins.
 // A sequence's shared partial page is copied unless every other holder has
 // been listed, with such a page, before it: its last holder keeps it.
 __global__ __launch_bounds__(kPlanThreads) void pa_pages_extend_plan_kernel(const Extend e) {
   __shared__ int scratch[kPlanThreads / 64];
-  __shared__ int ls[kMaxExtend], lp[kMaxExtend];
+  __shared__ __align__(16) int list[kMaxExtend];
+  __shared__ int before[kMaxExtend];
   if ((int)blockIdx.x < e.pool.chunks) {
     count_chunk(e.t.refs, e.t.pages, e.pool, blockIdx.x, scratch);
     return;
   }
-  for (int i = threadIdx.x; i < e.n; i += kPlanThreads) ls[i] = e.seqs[i];
-  __syncthreads();
   constexpr int kPer = kMaxExtend / kPlanThreads;
-  int need[kPer], len[kPer], share[kPer];
+  int need[kPer], len[kPer], share[kPer], held[kPer];
   // a thread's sequences are consecutive, so that its sums are in list order
-  const int per = (e.n + kPlanThreads - 1) / kPlanThreads;
+  const int per = (e.n + kPlanThreads - 1) / kPlanThreads, i0 = (int)threadIdx.x * per;
+  const int mine = pa_max(pa_min(per, e.n - i0), 0);
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
-    const int i = (int)threadIdx.x * per + k;
-    need[k] = -1;
-    share[k] = -1;
-    len[k] = 0;
-    if (k >= per || i >= e.n) continue;
-    const int s = ls[i], want = e.new_lengths[i];
-    bool ok = s >= 0 && s < e.t.rows;
-    for (int j = 0; j < i; ++j) ok &= ls[j] != s;
-    if (ok) {
-      len[k] = e.t.lengths[s];
-      ok = len[k] >= 0 && want >= len[k] && want <= (int64_t)e.t.width << e.t.lbs;
-    }
-    if (ok) {
-      need[k] = pages_of(e.t, want) - pages_of(e.t, len[k]);
-      if (want > len[k] && (len[k] & ((1 << e.t.lbs) - 1))) {
-        const int p = page_at(e.t, s, len[k] >> e.t.lbs);
-        if (p >= 0 && e.t.refs[p] > 1) share[k] = p;
+    need[k] = share[k] = -1;
+    len[k] = held[k] = 0;
+    if (k >= mine) continue;
+    const int s = e.seqs[i0 + k], want = e.new_lengths[i0 + k];
+    const bool in = s >= 0 && s < e.t.rows;
+    list[i0 + k] = in ? s : -1;
+    if (!in) continue;
+    len[k] = e.t.lengths[s];
+    if (len[k] < 0 || want < len[k] || want > (int64_t)e.t.width << e.t.lbs) continue;
+    need[k] = pages_of(e.t, want) - pages_of(e.t, len[k]);
+    if (want > len[k] && (len[k] & ((1 << e.t.lbs) - 1))) {
+      const int p = page_at(e.t, s, len[k] >> e.t.lbs);
+      if (p >= 0) {
+        held[k] = e.t.refs[p];
+        if (held[k] > 1) share[k] = p;
       }
     }
-    lp[i] = share[k];
   }
   __syncthreads();
-  int mine = 0;
+  count_before(list, e.n, before);
+  bool any = false;
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
-    const int i = (int)threadIdx.x * per + k;
-    if (share[k] >= 0) {
-      int rank = 0;
-      for (int j = 0; j < i; ++j) rank += lp[j] == share[k];
-      if (rank < e.t.refs[share[k]] - 1)
+    if (k >= mine) continue;
+    if (before[i0 + k]) need[k] = share[k] = -1;  // named before
+    any |= share[k] >= 0;
+  }
+  any = __syncthreads_or(any);
+  if (any) {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+      if (k < mine) list[i0 + k] = share[k];
+    __syncthreads();
+    count_before(list, e.n, before);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      if (k >= mine || share[k] < 0) continue;
+      if (before[i0 + k] < held[k] - 1)
         need[k] += 1;
       else
         share[k] = -1;
     }
-    mine += pa_max(need[k], 0);
   }
+  int sum = 0;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) sum += pa_max(need[k], 0);
   int total;
-  int at = block_before<kPlanThreads>(mine, &total, scratch);
+  int at = block_before<kPlanThreads>(sum, &total, scratch);
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
-    const int i = (int)threadIdx.x * per + k;
-    if (k >= per || i >= e.n) continue;
-    e.start[i] = need[k] >= 0 ? at : -1;
-    e.old[i] = len[k];
-    e.src[i] = share[k];
+    if (k >= mine) continue;
+    e.start[i0 + k] = need[k] >= 0 ? at : -1;
+    e.old[i0 + k] = len[k];
+    e.src[i0 + k] = share[k];
     at += pa_max(need[k], 0);
   }
 }
