@@ -22,6 +22,7 @@
 #include <vector>
 
 #include "pa_fp8.h"
+#include "sp_plan.h"
 
 namespace {
 
@@ -819,9 +820,9 @@ PyObject* shared_prefix(PyObject*, PyObject* const* a, Py_ssize_t n) {
     else NOT_HERE;
     const int64_t B = cl.size(0), G = pl.size(0), rows = q.size(0), Hq = q.size(1), D = q.size(2), NB = kc.size(0),
                   H = kc.size(1), bs = kc.size(3), M = bt.size(1);
-    if (B <= 0 || B > 4096 || G > 1024 || rows == 0 || rows % B || H <= 0 || Hq <= 0 || Hq % H || NB <= 0 || M <= 0)
+    if (B <= 0 || rows == 0 || rows % B || H <= 0 || Hq <= 0 || Hq % H || NB <= 0 || M <= 0)
       NOT_HERE;
-    if (D % 64 || D < 64 || D > 256 || bs < 16 || bs > 1024 || (bs & (bs - 1))) NOT_HERE;
+    if (D % 64 || D < 64 || D > 256 || B > sp_max_seqs((int)D) || G > sp_max_groups((int)D) || bs < 16 || bs > 1024 || (bs & (bs - 1))) NOT_HERE;
     const int64_t lim = 0x7fffffff;
     if (rows > lim || NB > lim || M > lim || Hq > lim) NOT_HERE;
     if (!shape_is(kc, {NB, H, D / 16, bs, 16})) NOT_HERE;

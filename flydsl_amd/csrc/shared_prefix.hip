@@ -153,7 +153,7 @@ struct Plan {
   int* row_tiles;     // [G + 1] prefix items of the groups before g, one kv head
 };
 
-__host__ __device__ inline int plan_bytes(int B, int G) {
+__host__ __device__ constexpr int plan_bytes(int B, int G) {
   return (8 * (B + 1) + 8 * (G + 1) + 8 * SP_WAVES + 8 * B + 12 * (G + 1) + 15) & ~15;
 }
 __device__ __forceinline__ Plan plan_of(char* lds, int B, int G) {
@@ -312,6 +312,7 @@ struct Piece {
   int row0, nrows;   // first row of the item among the group's rows (the sequence's columns), and their count
   int h;             // kv head
   int begin, end;    // tokens of the item
+  int seen;          // the first token behind those that any of its rows sees or that its sequences hold
   int tile, tile_end;  // tiles of the piece
   int rows_out;      // rows of a slot
   float* ml;         // the slot
@@ -389,6 +390,14 @@ struct Walk {
         pc.nrows = prefix ? __builtin_amdgcn_readfirstlane((pl.first[of + 1] - pl.first[of]) * s.eq) : s.eq;
         pc.begin = begin;
         pc.end = end;
+        pc.seen = end;
+        if (prefix) {
+          int most = 0;
+          const int b1 = (pa_min(pc.row0 + sh.rows, pc.nrows) - 1) / s.eq;
+          for (int b = pc.row0 / s.eq + (int)(threadIdx.x & 63); b <= b1; b += 64) most = pa_max(most, pl.ctx[pc.b0 + b]);
+          for (int d = 1; d < 64; d *= 2) most = pa_max(most, __shfl_xor(most, d, 64));
+          pc.seen = __builtin_amdgcn_readfirstlane(pa_min(end, most));
+        }
         pc.tile = begin / SP_TILE + t0;
         pc.tile_end = begin / SP_TILE + t1;
         pc.rows_out = prefix ? s.p_rows : s.s_rows;
@@ -756,7 +765,7 @@ __device__ __forceinline__ void run_direct(const SpArgs& s, const Piece& pc, con
     }
     // ---- masks: the part's first and last tiles ----
     const int t0 = tile * SP_TILE;
-    if (t0 < pc.begin || t0 + SP_TILE > pa_min(w.least, pc.end)) {
+    if (t0 < pc.begin || t0 + SP_TILE > pa_min(w.least, pc.seen)) {
       asm volatile("");  // (a branch: not computed for every tile)
 #pragma unroll
       for (int T = 0; T < 4; ++T)
@@ -765,10 +774,10 @@ __device__ __forceinline__ void run_direct(const SpArgs& s, const Piece& pc, con
           const int t = t0 + 16 * g + 4 * T + i;
           if (t < pc.begin || t >= w.limit[0]) l[T][0][i] = kNegInf;
         }
-      // bytes behind the part's tokens may be anything, NaN among it
+      // bytes behind the tokens may be anything, NaN among it
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int keep = (int)keep4(t0 + 16 * g + 4 * i, pc.begin, pc.end);
+        const int keep = (int)keep4(t0 + 16 * g + 4 * i, pc.begin, pc.seen);
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) x.v[dt][i] &= keep;
       }
@@ -778,7 +787,7 @@ __device__ __forceinline__ void run_direct(const SpArgs& s, const Piece& pc, con
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int t = t0 + 16 * g + 4 * T + i;
-            if (t < pc.begin || t >= pc.end) vs[T][i] = 0.0f;
+            if (t < pc.begin || t >= pc.seen) vs[T][i] = 0.0f;
           }
       }
     }
@@ -820,6 +829,9 @@ __host__ __device__ constexpr int tile_bytes(int d) {
 __host__ __device__ constexpr int work_bytes(int d, bool shared) {
   return shared ? 2 * tile_bytes(d) : 0;
 }
+
+constexpr bool lds_fits(int d, int seqs) { return plan_bytes(seqs, seqs / 4) + work_bytes(d, true) <= 160 * 1024; }
+static_assert(lds_fits(64, 4096) && lds_fits(128, 4096) && lds_fits(192, 2048) && lds_fits(256, 512), "sp_max_seqs");
 
 // Masks of the scheduling groups.
 constexpr int kSchedAlu = 0x2, kSchedMfma = 0x8, kSchedDsRead = 0x100, kSchedDsWrite = 0x200;
@@ -865,17 +877,17 @@ __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, con
   };
   auto mask = [&](int tile) {
     const int t0 = tile * SP_TILE;
-    if (t0 < pc.begin || t0 + SP_TILE > pc.end) {  // bytes outside the part may be anything, NaN among it
+    if (t0 < pc.begin || t0 + SP_TILE > pc.seen) {  // bytes behind the tokens may be anything, NaN among it
       asm volatile("");
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int keep = (int)keep4(t0 + 16 * wave + 4 * k, pc.begin, pc.end);
+        const int keep = (int)keep4(t0 + 16 * wave + 4 * k, pc.begin, pc.seen);
 #pragma unroll
         for (int i = 0; i < NS; ++i) vst[i][k] &= keep;
       }
       if constexpr (PT) {
         const int t = t0 + 16 * wave + c;
-        if (t < pc.begin || t >= pc.end) sst = 0.0f;
+        if (t < pc.begin || t >= pc.seen) sst = 0.0f;
       }
     }
   };
@@ -1202,7 +1214,7 @@ bool head_ok(int d) { return d == 64 || d == 128 || d == 192 || d == 256; }
 // Sizes of a launch; 0 or a PA_ERR_* code.
 int sizes_of(int B, int G, int H, int ql, int gqa, int D, int workers, Sizes* z) {
   if (!head_ok(D)) return PA_ERR_HEAD_SIZE;
-  if (B < 0 || G < 0 || H <= 0 || ql <= 0 || gqa <= 0 || workers <= 0 || B > SP_MAX_SEQS || G > SP_MAX_GROUPS)
+  if (B < 0 || G < 0 || H <= 0 || ql <= 0 || gqa <= 0 || workers <= 0 || B > sp_max_seqs(D) || G > sp_max_groups(D))
     return PA_ERR_SHAPE;
   const int64_t eq = (int64_t)ql * gqa, rows = eq * B;
   if (eq > (1 << 20) || rows > 0x7fffffff || (int64_t)H * gqa > 0x7fffffff) return PA_ERR_SHAPE;

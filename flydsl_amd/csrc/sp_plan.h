@@ -23,10 +23,14 @@
 
 #define SP_TILE 64          // tokens of a tile
 #define SP_WAVES 4          // waves of a workgroup
-#define SP_MAX_SEQS 4096    // the plan of a launch is held in LDS
-#define SP_MAX_GROUPS 1024
 #define SP_MAX_TOKENS (1 << 30)  // of a table row: larger ones count as this
 #define SP_MIN_SHARE 160         // at least a shared tile, and four of a wave's pieces
+
+// Sequences and groups of a launch, whose plan (16 bytes a sequence, 20 a group)
+// is held in LDS beside two buffers of a tile: 73 KB of the 160 at head size 128,
+// 109 at 192, 145 at 256.
+PA_HD int sp_max_seqs(int head_size) { return head_size <= 128 ? 4096 : head_size <= 192 ? 2048 : 512; }
+PA_HD int sp_max_groups(int head_size) { return sp_max_seqs(head_size) / 4; }
 
 typedef struct SpShape {
   int shared;    // tiles come through LDS to a workgroup; else a wave works alone

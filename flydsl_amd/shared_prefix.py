@@ -10,10 +10,10 @@ pa_decode_ps_launch (kernels/pa_decode_fp8.py:2812-3202).
 Groups: sequences ``prefix_indptr[g] .. prefix_indptr[g + 1] - 1`` have the same
 first ``prefix_lengths[g]`` tokens, as sequences forked off one prompt have
 (:func:`flydsl_amd.fork_cache_pages`).  They are read through the block-table
-row of the group's first sequence; the tokens behind them through each
-sequence's own row.  The shared length need not end with a page.  Sequences
-before, between (groups of length 0) and behind the groups are decoded by
-themselves.
+row of the group's first sequence, which has to hold their pages whatever its
+own context length; the tokens behind them through each sequence's own row.
+The shared length need not end with a page.  Sequences before, between (groups
+of length 0) and behind the groups are decoded by themselves.
 """
 
 from __future__ import annotations
@@ -35,8 +35,7 @@ from .pa_decode import (
 
 ROUTE = "ps_shared_prefix"
 HEAD_SIZES = (64, 128, 192, 256)
-MAX_SEQS = 4096
-MAX_GROUPS = 1024
+MAX_SEQS = {64: 4096, 128: 4096, 192: 2048, 256: 512}  # by head size; a quarter as many groups
 
 
 def _workers(device) -> int:
@@ -103,7 +102,8 @@ def pa_decode_shared_prefix(
     [1] tensor or [NB, Hkv, bs, 1].  Query token i of a sequence of n tokens
     sees keys 0 .. n - ql + i; a row that sees none is zero.  head_dim 64,
     128, 192 or 256, page size 16 to 1024 (a power of two), any query_length x
-    group size, up to 4096 sequences and 1024 groups.  Returns the route name.
+    group size, up to 4096 sequences and 1024 groups (head_dim 192: 2048 and 512;
+    256: 512 and 128).  Returns the route name.
     Under graph capture the scales must be float32 device tensors.
     """
     native = _lib.native()
@@ -197,8 +197,9 @@ def prepare_pa_decode_shared_prefix(
         raise ValueError(f"block_tables has {block_tables.shape[0]} rows for {b} sequences")
     if prefix_indptr.shape[0] != g + 1:
         raise ValueError(f"prefix_indptr must have {g + 1} entries for {g} groups, got {prefix_indptr.shape[0]}")
-    if b > MAX_SEQS or g > MAX_GROUPS:
-        raise NotImplementedError(f"at most {MAX_SEQS} sequences and {MAX_GROUPS} groups, got {b} and {g}")
+    if b > MAX_SEQS[d] or g > MAX_SEQS[d] // 4:
+        raise NotImplementedError(f"at most {MAX_SEQS[d]} sequences and {MAX_SEQS[d] // 4} groups with head_dim={d}, got "
+                                  f"{b} and {g}")
 
     a = _lib.SharedPrefixArgs()
     if b == 0:

@@ -622,14 +622,15 @@ int pa_fp8_fnuz_to_fn(const void* src, const int32_t* rows, int64_t num_rows, in
  * qi of a sequence of n tokens sees keys 0 .. n - ql + qi).  Group g is the
  * sequences prefix_indptr[g] .. prefix_indptr[g + 1] - 1, whose first
  * prefix_lengths[g] tokens are the same: they are read once for the group,
- * through the table row of its first sequence, the tokens behind them through
- * each sequence's own row.  Any prefix length is taken (it need not end with a
+ * through the table row of its first sequence (whatever that sequence's own
+ * length), the tokens behind them through each sequence's own row.  Any prefix length is taken (it need not end with a
  * page); sequences outside the groups share nothing.  Group bounds are clamped
  * to [0, num_seqs] and to never fall, lengths to what a table row can hold.
  * Rows that see no key are zero.
  *
  * Head sizes 64, 128, 192 and 256; page sizes 16, 32, ..., 1024 (powers of
- * two); at most 4096 sequences and 1024 groups.  Two launches; the workspace
+ * two); at most 4096 sequences and 1024 groups (head size 192: 2048 and 512,
+ * 256: 512 and 128).  Two launches; the workspace
  * (pa_fp8_shared_prefix_workspace_bytes) needs no initialisation and is the
  * call's own until the launches end.  num_workers: persistent workgroups, two
  * per compute unit.  16-byte alignment: query strides are multiples of 8

@@ -7,9 +7,12 @@ import numpy as np
 import pytest
 import torch
 
-from flydsl_amd import compact_cache_pages, copy_cache_pages, extend_cache_pages, fork_cache_pages, free_cache_pages
+from flydsl_amd import (_lib, compact_cache_pages, copy_cache_pages, extend_cache_pages, fork_cache_pages,
+                        free_cache_pages)
 from oracle import cache_pages as oracle
 from tests._page_cases import make_caches, make_pool
+from tests.test_gpu_checked import checked  # noqa: F401 (a fixture)
+from tests.test_gpu_native import both
 
 pytestmark = pytest.mark.gpu
 
@@ -274,3 +277,46 @@ def test_streams_and_graphs():
         assert agree()
         free_cache_pages(a.dt, a.dn, a.dr, dev([2]), bs, new_lengths=dev([0]))
         free_cache_pages(b.dt, b.dn, b.dr, dev([2]), bs, new_lengths=dev([0]))
+
+
+def test_native_path_gives_the_same_bits(monkeypatch):
+    bs = 16
+    s = State(*make_pool(12, 8, 60, bs, seed=8, empty=6), bs)
+    old = [x.clone() for x in (s.dt, s.dn, s.dr, *s.dc)]
+
+    def run_all():
+        for x, o in zip((s.dt, s.dn, s.dr, *s.dc), old):
+            x.copy_(o)
+        a = fork_cache_pages(s.dt, s.dn, s.dr, dev([0, 1, 99]), dev([6, 7, 8]), bs)
+        b = extend_cache_pages(s.dc, s.dt, s.dn, s.dr, dev([6, 7]), s.dn[[0, 1]] + 9, bs)
+        c = copy_cache_pages(s.dc, dev([0, 1]), dev([58, 59]))
+        d = free_cache_pages(s.dt, s.dn, s.dr, dev([0, 2]), bs, new_lengths=s.dn[[0, 2]] // 2)
+        e = free_cache_pages(s.dt, s.dn, s.dr, dev([3]), bs)
+        f = compact_cache_pages(s.dc, s.dt, s.dn, s.dr, bs)
+        return [x.clone() for x in (a, b, c, d, e, *f, s.dt, s.dn, s.dr)] + [x.view(torch.uint8).clone() for x in s.dc]
+
+    both(monkeypatch, run_all)
+
+
+def test_checked_build(checked, monkeypatch):
+    """Table entries outside the cache are passed over and noted."""
+    monkeypatch.setattr(_lib, "_NATIVE", False)  # (bound to the release library)
+    t, n, refs = make_pool(8, 6, 64, 16, seed=9, empty=3)
+    s = State(t, n, refs, 16)
+    s.fork([0, 1], [5, 6])
+    s.extend([5, 6], [int(n[0]) + 3, int(n[1]) + 20])
+    s.compact()
+    assert _lib.debug_violations(checked) == 0
+    t, n = np.array([[3, 99, 5], [7, -2, 0], [0, 0, 0]], np.int32), np.array([40, 20, 0], np.int32)
+    refs = np.zeros(9, np.int32)
+    refs[[3, 5, 7]] = 1
+    s = State(t, n, refs, 16)
+    s.fork([0], [2])
+    assert _lib.debug_violations(checked) == _lib.VIOLATION_PAGE
+    s.extend([1, 2], [30, 41])
+    assert _lib.debug_violations(checked) == _lib.VIOLATION_PAGE
+    s.compact()
+    assert _lib.debug_violations(checked) == _lib.VIOLATION_PAGE
+    s.free([0, 1, 2])
+    assert _lib.debug_violations(checked) == _lib.VIOLATION_PAGE
+    assert not s.refs.any()

@@ -21,9 +21,11 @@ from __future__ import annotations
 import pytest
 import torch
 
-from flydsl_amd import pa_decode_ps_launch, pa_decode_shared_prefix, prepare_pa_decode_shared_prefix
+from flydsl_amd import _lib, pa_decode_ps_launch, pa_decode_shared_prefix, prepare_pa_decode_shared_prefix
 from oracle import shared_prefix as oracle
 from tests._prefix_cases import make_prefix_case
+from tests.test_gpu_checked import checked  # noqa: F401 (a fixture)
+from tests.test_gpu_native import both
 
 pytestmark = pytest.mark.gpu
 
@@ -244,3 +246,135 @@ def test_empty_batch_and_refusals_on_the_device():
     q = torch.empty(d["query"].numel() + 4, dtype=torch.bfloat16, device=DEV)[4:].view(d["query"].shape)
     with pytest.raises(RuntimeError, match="PA_ERR_ALIGN"):
         call(dict(d, query=q), torch.empty_like(d["query"]))
+
+
+@pytest.mark.parametrize("G", [63, 64, 65, 300])
+def test_many_groups(G):
+    """Groups on both sides of what one wave plans, some of them empty or of no
+    shared token, and sequences before and behind them."""
+    lens = [(0 if g % 11 == 3 else 5 + 7 * (g % 13), 0 if g % 7 == 5 else 1 + g % 3) for g in range(G)]
+    case = make_prefix_case(groups=[(p if k else 0, [p + 1 + 5 * j for j in range(k)]) for p, k in lens],
+                            loose=[40, 0, 90], heads=4, kv_heads=1, head=64, seed=G)
+    run(case)
+
+
+@pytest.mark.parametrize("head,B", [(64, 4096), (128, 4096), (192, 2048), (256, 512)])
+def test_most_sequences_and_groups(head, B):
+    """As many as a call takes: the whole plan beside the tiles."""
+    groups = [(3 + g % 29, [3 + g % 29 + (g + j) % 40 for j in range(4)]) for g in range(B // 4)]
+    run(make_prefix_case(groups=groups, heads=2, kv_heads=1, head=head, seed=head, spare_pages=1))
+
+
+def test_bounds_and_lengths_out_of_range():
+    """Group bounds that fall or pass the batch, negative lengths and such past
+    a table row count as the nearest ones in range."""
+    case = make_prefix_case(groups=[ragged(200, 3, 20, 1), ragged(100, 3, 20, 1)], loose=[50, 60], seed=21,
+                            poison=False)
+    d = to_dev(case)
+    cap = d["block_tables"].shape[1] * 16
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    for given, meant in (
+        (dict(prefix_indptr=i32(-5, 3, 2), prefix_lengths=i32(200, 50)),
+         dict(prefix_indptr=i32(0, 3, 3), prefix_lengths=i32(200, 0))),
+        (dict(prefix_indptr=i32(3, 2**31 - 1, 3), prefix_lengths=i32(40, 7)),
+         dict(prefix_indptr=i32(3, 8, 8), prefix_lengths=i32(40, 0))),
+        (dict(prefix_lengths=i32(-3, -2**31)), dict(prefix_lengths=i32(0, 0))),
+        (dict(prefix_lengths=i32(2**31 - 1, 100)), dict(prefix_lengths=i32(cap, 100))),
+        (dict(context_lengths=i32(-4, -2**31, 2**31 - 1, 100, 50, 40, 30, 20)),
+         dict(context_lengths=i32(0, 0, cap, 100, 50, 40, 30, 20))),
+    ):
+        e, m = dict(d, **given), dict(d, **meant)
+        out = torch.full_like(e["query"], float("nan"))
+        call(e, out)
+        check(m, out)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(heads=32, kv_heads=2), dict(per_token=True), dict(head=64, trans=False)])
+def test_shared_tokens_that_no_one_sees(kw):
+    """A prefix longer than every context of its group, with NaN behind them
+    (a page not written yet); a group whose sequences have all ended."""
+    case = make_prefix_case(groups=[(300, [301, 100, 20, 130]), (90, [91, 90])], seed=22, **kw)
+    ctx = [0, 100, 20, 130, 0, 0]
+    bt, v = case["block_tables"], case["value_cache"].view(torch.uint8)
+    for t in range(130, 300):
+        p, o = int(bt[0, t // 16]), t % 16
+        if v.dim() == 5:
+            v[p, :, o // 16, :, o % 16] = 0x7F
+        else:
+            v[p, :, :, o] = 0x7F
+        if kw.get("per_token"):
+            case["value_scale"][p, :, o] = float("inf")
+            case["key_scale"][p, :, o] = float("nan")
+    run(dict(case, context_lengths=torch.tensor(ctx, dtype=torch.int32)))
+
+
+def test_a_sequence_of_nan_leaves_the_others_alone():
+    case = make_prefix_case(groups=[ragged(100, 40, 5, 20)], heads=8, kv_heads=2, seed=23)
+    d = to_dev(case)
+    want = reference(d)
+    own = int(case["block_tables"][7, int(case["context_lengths"][7] - 1) // 16])
+    d["value_cache"].view(torch.uint8)[own] = 0x7F
+    out = torch.empty_like(d["query"])
+    call(d, out)
+    assert torch.isnan(out[7].float()).all()
+    keep = [r for r in range(40) if r != 7]
+    sub = dict(d, query=d["query"][keep])
+    check(sub, out[keep], tuple(x[keep] for x in want))
+
+
+@pytest.mark.parametrize("per_token", [False, True])
+def test_offsets_past_32_bits(per_token):
+    """Pages more than 4 GiB apart."""
+    case = make_prefix_case(groups=[ragged(700, 4, 60, 1)], heads=8, kv_heads=2, per_token=per_token, page=64, seed=24)
+    d = to_dev(case)
+    nb = d["key_cache"].shape[0]
+    step = -(-(5 << 30) // nb) // 1024 * 1024
+    big = torch.empty(nb * step, dtype=torch.uint8, device=DEV)
+    at = 0
+    for name in ("key_cache", "value_cache", "key_scale", "value_scale"):
+        t = d[name]
+        if t.dim() < 4:
+            continue
+        raw = t.view(torch.uint8).flatten(1)
+        view = big.view(nb, step)[:, at: at + raw.shape[1]]
+        view.copy_(raw)
+        at += raw.shape[1]
+        d[name] = view.view(t.dtype).unflatten(1, t.shape[1:])
+    assert d["key_cache"].stride(0) == step and (nb - 1) * step > 1 << 32
+    out = torch.empty_like(d["query"])
+    call(d, out)
+    check({**to_dev(case)}, out)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(groups=[ragged(300, 5, 30, 1)], loose=[70]),
+    dict(groups=[ragged(300, 5, 30, 4)], ql=4, heads=16, kv_heads=2, per_token=True, dtype=torch.float16, page=64),
+    dict(groups=[ragged(200, 3, 30, 1)], trans=False, head=64),
+    dict(groups=[], loose=[5, 6]),
+])
+def test_native_path_gives_the_same_bits(monkeypatch, kw):
+    d = to_dev(make_prefix_case(**kw, seed=25))
+
+    def both_ways():
+        out = torch.full_like(d["query"], 3.0)
+        return call(d, out), out
+
+    both(monkeypatch, both_ways)
+
+
+@pytest.mark.parametrize("kw", [dict(heads=8, kv_heads=2), dict(heads=32, kv_heads=2),
+                                dict(heads=8, kv_heads=2, per_token=True)])
+def test_checked_build(checked, monkeypatch, kw):
+    """Clean calls note nothing; table entries outside the cache are read as the
+    nearest page and noted."""
+    monkeypatch.setattr(_lib, "_NATIVE", False)  # (bound to the release library)
+    case = make_prefix_case(groups=[ragged(200, 6, 40, 1)], loose=[90], seed=26, poison=False, **kw)
+    run(case)
+    assert _lib.debug_violations(checked) == 0
+    bt, nb = case["block_tables"].clone(), case["key_cache"].shape[0]
+    bt[0, 3], bt[4, 14], bt[6, 2] = -9, nb + 5, 2**31 - 1
+    d = to_dev(dict(case, block_tables=bt))
+    out = torch.empty_like(d["query"])
+    call(d, out)
+    check(dict(d, block_tables=d["block_tables"].clamp(0, nb - 1)), out)
+    assert _lib.debug_violations(checked) == _lib.VIOLATION_PAGE

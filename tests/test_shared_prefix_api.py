@@ -97,6 +97,10 @@ def test_refusals():
     many = torch.zeros(5000, dtype=torch.int32)
     bad("at most 4096", NotImplementedError, query=torch.empty(5000, 8, 128, dtype=torch.bfloat16),
         context_lengths=many, block_tables=many[:, None])
+    wide = make_prefix_case(groups=[(10, [12])], head=256, page=32)
+    with pytest.raises(NotImplementedError, match="at most 512"):
+        prep(wide, query=torch.empty(513, 8, 256, dtype=torch.bfloat16), context_lengths=many[:513],
+             block_tables=many[:513, None])
     with pytest.raises(RuntimeError, match="must be on a GPU"):
         prepare_pa_decode_shared_prefix(torch.empty_like(c["query"]), *[c[k] for k in (
             "query", "key_cache", "value_cache", "context_lengths", "block_tables", "prefix_indptr", "prefix_lengths",

@@ -124,5 +124,7 @@ def test_refusals():
 
     assert "PA_ERR_HEAD_SIZE" in code(4, 1, 2, 1, 4, 96, 256)
     for bad in ((4097, 1, 2, 1, 4, 128, 256), (4, 1025, 2, 1, 4, 128, 256), (4, 1, 0, 1, 4, 128, 256),
-                (4, 1, 2, 0, 4, 128, 256), (4, 1, 2, 1, 0, 128, 256), (4, 1, 2, 1, 4, 128, 0)):
+                (4, 1, 2, 0, 4, 128, 256), (4, 1, 2, 1, 0, 128, 256), (4, 1, 2, 1, 4, 128, 0),
+                (2049, 1, 2, 1, 4, 192, 256), (4, 513, 2, 1, 4, 192, 256), (513, 1, 2, 1, 4, 256, 256),
+                (4, 129, 2, 1, 4, 256, 256)):
         assert "PA_ERR_SHAPE" in code(*bad)
