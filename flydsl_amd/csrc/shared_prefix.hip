@@ -433,11 +433,9 @@ struct Walk {
 };
 
 // LDS behind the plan, of shared items: two buffers of a tile, or, at a piece's
-// end, maxima and sums by wave and 32 output dims of every row.
-constexpr int kOutStride = 36;  // floats a row of 32 dims takes (16-byte steps that spread over the banks)
-__host__ __device__ constexpr int end_bytes(int nr) {
-  return SP_WAVES * 16 * nr * 4 * 2 + SP_WAVES * 16 * nr * kOutStride * 4;
-}
+// end, maxima, sums and outputs of every wave's rows.
+__host__ __device__ constexpr int out_stride(int d) { return d + 4; }  // floats (16-byte steps that spread over the banks)
+__host__ __device__ constexpr int end_bytes(int d, int nr) { return SP_WAVES * 16 * nr * (2 + out_stride(d)) * 4; }
 
 // The wave's rows: operand B of the key product, the keys each row sees, and
 // their softmax.
@@ -597,7 +595,7 @@ struct Rows {
   __device__ __forceinline__ void finish(const Piece& pc, char* lds, int wt, int wave, int wr, int wi, int c, int g) {
     float* lm = (float*)lds;              // [wave][16 NR]
     float* ll = lm + SP_WAVES * 16 * NR;
-    float* lo = ll + SP_WAVES * 16 * NR;  // [wave][16 NR][kOutStride]
+    float* lo = ll + SP_WAVES * 16 * NR;  // [wave][16 NR][out_stride]
     __syncthreads();                      // what LDS held before has been read
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
@@ -626,24 +624,21 @@ struct Rows {
         pc.ml[pc.rows_out + r] = all;
       }
     }
-    const int rows = SP_WAVES / wt * 16 * NR;
 #pragma unroll
-    for (int d0 = 0; d0 < D / 32; ++d0) {
-      if (d0) __syncthreads();
+    for (int n = 0; n < NR; ++n)
 #pragma unroll
-      for (int n = 0; n < NR; ++n)
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          *(f32x4*)(lo + ((wave * NR + n) * 16 + c) * kOutStride + 16 * k + 4 * g) = o[n][2 * d0 + k];
-      __syncthreads();
-      for (int i = threadIdx.x; i < rows * 8; i += kThreads) {
-        const int r = i >> 3, d = (i & 7) * 4;
-        if (pc.row0 + r >= pc.nrows) break;  // (rows only grow with i)
-        const int w0 = r / (16 * NR) * wt, rr = r % (16 * NR);
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        for (int w = w0; w < w0 + wt; ++w) v += *(const f32x4*)(lo + (w * 16 * NR + rr) * kOutStride + d);
-        *(f32x4*)(pc.o + (int64_t)r * D + 32 * d0 + d) = v;
-      }
+      for (int dt = 0; dt < D / 16; ++dt)
+        *(f32x4*)(lo + ((wave * NR + n) * 16 + c) * out_stride(D) + 16 * dt + 4 * g) = o[n][dt];
+    __syncthreads();
+    // whole rows, so that a wave's stores are of whole kilobytes
+    const int rows = pa_min(SP_WAVES / wt * 16 * NR, pc.nrows - pc.row0);
+#pragma unroll 4
+    for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
+      const int r = i / (D / 4), d = i % (D / 4) * 4;
+      const int w0 = r / (16 * NR) * wt, rr = r % (16 * NR);
+      f32x4 v = *(const f32x4*)(lo + (w0 * 16 * NR + rr) * out_stride(D) + d);
+      if (wt == 2) v += *(const f32x4*)(lo + ((w0 + 1) * 16 * NR + rr) * out_stride(D) + d);
+      *(f32x4*)(pc.o + 4 * i) = v;
     }
     __syncthreads();  // LDS is the next piece's
   }
@@ -860,9 +855,10 @@ __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, con
   const uint32_t k_step = (uint32_t)(bs * 64), v_step = (uint32_t)(64 * v_dim);
   i32x4 kst[NS], vst[NS];
   float sst = 0.0f;
-  int page = 0;
-  auto next_page = [&](int tile) { page = page_of(tile * SP_TILE + 16 * wave); };
-  auto fetch = [&](int tile) {
+  const int last = pc.tile_end - 1;
+  auto page_at = [&](int tile) { return page_of.entry(pa_min(tile, last) * SP_TILE + 16 * wave); };
+  auto fetch = [&](int tile, int entry) {
+    const int page = Pages::inside(entry, a.num_blocks);
     const int in = (tile * SP_TILE + 16 * wave) & (bs - 1);
     const uint8_t* kp = kbase + (int64_t)page * a.stride_k_block + in * 16;
     const uint8_t* vp = vbase + (int64_t)page * a.stride_v_block + (in >> 4) * v_blk;
@@ -912,22 +908,22 @@ __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, con
     }
   };
 
-  next_page(pc.tile);
+  // (two rounds of loads: table entries and queries, then the first tile)
+  int entry = page_at(pc.tile), entry1 = page_at(pc.tile + 1);
   Rows<D, F16, PT, NR> w;
   w.set_scale(s);
   {
     i32x4 x[NR][D / 32];
 #pragma unroll
     for (int n = 0; n < NR; ++n) w.template load_query<false>(s, pc, pc.row0 + (wr * NR + n) * 16 + c, g, x[n]);
+    fetch(pc.tile, entry);
 #pragma unroll
     for (int n = 0; n < NR; ++n) w.begin(s, pc, ctx, n, pc.row0 + (wr * NR + n) * 16 + c, x[n]);
   }
-  fetch(pc.tile);
-  next_page(pa_min(pc.tile + 1, pc.tile_end - 1));
+  entry = page_at(pc.tile + 2);
   mask(pc.tile);
   store(0);
-  fetch(pa_min(pc.tile + 1, pc.tile_end - 1));
-  next_page(pa_min(pc.tile + 2, pc.tile_end - 1));
+  fetch(pa_min(pc.tile + 1, last), entry1);
   __syncthreads();
   int buffer = 0;
   for (int tile = pc.tile; tile < pc.tile_end; ++tile, buffer ^= 1) {
@@ -1013,7 +1009,7 @@ __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, con
     }
     // the last product beside the next tile's way into LDS (behind the last tile:
     // once more the last, which no one reads)
-    mask(pa_min(tile + 1, pc.tile_end - 1));
+    mask(pa_min(tile + 1, last));
     __builtin_amdgcn_sched_barrier(0);
     w.add_sums(p);
 #pragma unroll
@@ -1030,14 +1026,16 @@ __device__ __forceinline__ void run_shared(const SpArgs& s, const Piece& pc, con
       __builtin_amdgcn_sched_group_barrier(kSchedAlu, 4, 0);
       __builtin_amdgcn_sched_group_barrier(kSchedDsWrite, 1, 0);
     }
-    fetch(pa_min(tile + 2, pc.tile_end - 1));
-    next_page(pa_min(tile + 3, pc.tile_end - 1));
+    if (tile + 2 <= last) fetch(tile + 2, entry);
+    entry = page_at(tile + 3);
     __syncthreads();
   }
   w.finish(pc, lds, WT, wave, wr, wi, c, g);
 }
 
-static_assert(end_bytes(2) <= 2 * tile_bytes(64), "a piece's end fits the tiles' buffers");
+static_assert(end_bytes(64, 2) <= 2 * tile_bytes(64) && end_bytes(128, 2) <= 2 * tile_bytes(128) &&
+                  end_bytes(192, 1) <= 2 * tile_bytes(192) && end_bytes(256, 1) <= 2 * tile_bytes(256),
+              "a piece's end fits the tiles' buffers");
 
 // ---------------------------------------------------------------------------
 // The kernels
