@@ -404,7 +404,7 @@ struct Walk {
         pc.ml = (prefix ? s.p_ml : s.s_ml) + (int64_t)slot * 2 * pc.rows_out;
         pc.o = (prefix ? s.p_o : s.s_o) + (int64_t)slot * pc.rows_out * D;
         if (t0 == 0 && (alone ? (threadIdx.x & 63) : threadIdx.x) == 0) {
-          const int last = t1 == n ? worker : sp_worker_of(i_at + sh.overhead + ((int64_t)(n - 1) << sh.lcost), share);
+          const int last = t1 == n ? worker : sp_worker_of(i_at + sh.overhead + (int64_t)(n - 1) * sh.cost, share);
           s.items[prefix ? item : s.max_prefix_items + item] = int2{slot, last - worker + 1};
         }
         return true;
@@ -1327,7 +1327,7 @@ extern "C" int pa_fp8_plan_shared_prefix(const int32_t* context_lengths, const i
     const int64_t q = sh.shared ? share : share / SP_WAVES;
     for (int i = 0; i < k.items; ++i) {
       const int w0 = sp_worker_of(at + sh.overhead, q);
-      const int w1 = sp_worker_of(at + sh.overhead + ((int64_t)(k.tiles - 1) << sh.lcost), q);
+      const int w1 = sp_worker_of(at + sh.overhead + (int64_t)(k.tiles - 1) * sh.cost, q);
       for (int w = w0; w <= w1; ++w) {
         const int t0 = k.begin / SP_TILE + sp_tile_from(sh, w * q, at, k.tiles);
         const int t1 = k.begin / SP_TILE + sp_tile_from(sh, (w + 1) * q, at, k.tiles);

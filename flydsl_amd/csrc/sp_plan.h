@@ -37,7 +37,7 @@ typedef struct SpShape {
   int nr;        // 16-row tiles of a wave
   int wt;        // waves that hold the same rows (shared)
   int rows;      // of an item
-  int lcost;     // log2 of a tile's cost, in eighths of a microsecond of one wave
+  int cost;      // of a tile, a shared one's being 64 (of a direct one, which a wave alone works, a quarter of its time)
   int overhead;  // of beginning and ending a piece
 } SpShape;
 
@@ -45,6 +45,14 @@ typedef struct SpShape {
 // tile beside them; up to twice what two waves hold, two waves share the rows
 // and split the tile's tokens; beyond, each wave has its own.  Two 16-row tiles
 // a wave where the head size leaves registers for them.
+//
+// Costs, from the times that workgroups with one kind of item took (two on a
+// CU): a shared tile 2.0 us, beginning and ending a shared piece 5 us.  A direct
+// tile moves half the bytes at head size 64.  Measured with the caches in HBM:
+// 256 sequences of a 16383-token prefix at head size 128 take 126 us with direct
+// tiles at 22, 129 at 26 and 138 at 16, 32 sequences of a 32768-token prefix 58.5,
+// 57 and 63 us; two prefixes at head size 64 take 34.0 us at 16, 34.9 at 18, 35.7
+// at 20.
 PA_HD SpShape sp_shape(int rows, int head_size) {
   const int most = head_size <= 128 ? 2 : 1;
   SpShape s;
@@ -52,7 +60,7 @@ PA_HD SpShape sp_shape(int rows, int head_size) {
   s.nr = rows > 32 ? most : 1;
   s.wt = !s.shared ? 1 : (rows > 32 * s.nr ? 1 : 2);
   s.rows = s.shared ? 16 * s.nr * (SP_WAVES / s.wt) : 16;
-  s.lcost = s.shared ? 6 : 4;
+  s.cost = s.shared ? 64 : head_size <= 64 ? 16 : 22;
   s.overhead = s.shared ? 160 : 40;
   return s;
 }
@@ -60,7 +68,7 @@ PA_HD SpShape sp_shape(int rows, int head_size) {
 PA_HD int sp_tiles(int first_token, int end_token) {
   return end_token <= first_token ? 0 : pa_cdiv(end_token, SP_TILE) - first_token / SP_TILE;
 }
-PA_HD int sp_item_cost(const SpShape& s, int tiles) { return tiles > 0 ? s.overhead + (tiles << s.lcost) : 0; }
+PA_HD int sp_item_cost(const SpShape& s, int tiles) { return tiles > 0 ? s.overhead + tiles * s.cost : 0; }
 
 // A workgroup's share of a line of shared and direct items: a multiple of four that
 // no worker's part of is shorter than a tile.  The direct items begin with a
@@ -86,6 +94,6 @@ PA_HD int64_t sp_direct_at(int64_t shared, int64_t share, int workers) {
 PA_HD int sp_tile_from(const SpShape& s, int64_t x, int64_t at, int tiles) {
   const int64_t d = x - at - s.overhead;
   if (d <= 0) return 0;
-  if (d > (int64_t)tiles << s.lcost) return tiles;
-  return (int)(((uint32_t)d + (1u << s.lcost) - 1) >> s.lcost);  // (a row's tiles times their cost: below 2^31)
+  if (d > (int64_t)tiles * s.cost) return tiles;
+  return (int)(((uint32_t)d + s.cost - 1) / (uint32_t)s.cost);  // (a row's tiles times their cost: below 2^31)
 }

@@ -112,7 +112,7 @@ def test_shares_are_even():
     pieces = check([17000 + i for i in range(256)], [0, 256], [16383], 8, 1, 4, 128, 1 << 20, 256)
     cost = np.zeros(256)
     for is_p, _, w, _, _, _, t0, t1 in pieces.tolist():
-        cost[w if is_p else w // 4] += 160 + (t1 - t0) * 64 if is_p else 40 + (t1 - t0) * 16
+        cost[w if is_p else w // 4] += 160 + (t1 - t0) * 64 if is_p else 40 + (t1 - t0) * 22
     assert cost.max() <= cost.mean() + 64 + 160
 
 
