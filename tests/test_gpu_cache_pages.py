@@ -146,7 +146,7 @@ def test_freeing_more_than_is_held():
     assert not s.refs.any()
 
 
-@pytest.mark.parametrize("n", [1, 5, 64, 65, 700])
+@pytest.mark.parametrize("n", [1, 5, 64, 65, 700, 2051])
 def test_copies(n):
     rng = np.random.default_rng(n)
     pages = 2 * n + 5
