@@ -22,7 +22,8 @@ Every operator decides on the state before the call and returns (compact
 aside) an int32 status a list entry: 1 carried out, 0 left out (an index or
 length out of range, an entry named before, a pool that has run out; see each
 function).  Pages are given out lowest index first in the order of the list,
-so results depend on nothing but the state.
+so results depend on nothing but the state.  Calls on one state have to follow
+each other on a stream.
 """
 
 from __future__ import annotations

@@ -632,7 +632,8 @@ int table_of(const pa_fp8_page_table_args* a, Table* t) {
   if (a->num_rows < 0 || a->max_blocks_per_seq < 0 || a->num_blocks < 0 || a->num_blocks > kMaxPages ||
       a->stride_bt_seq < 0)
     return PA_ERR_SHAPE;
-  if ((a->num_rows > 0 && (!a->block_tables || !a->context_lengths)) || (a->num_blocks > 0 && !a->ref_counts))
+  if ((a->num_rows > 0 && ((a->max_blocks_per_seq > 0 && !a->block_tables) || !a->context_lengths)) ||
+      (a->num_blocks > 0 && !a->ref_counts))
     return PA_ERR_NULL_ARG;
   t->tables = a->block_tables;
   t->stride = a->stride_bt_seq;
@@ -823,7 +824,8 @@ extern "C" int pa_fp8_compact_pages(const pa_fp8_page_table_args* a, const pa_fp
   int rc = table_of(a, &c.t);
   if (rc == PA_OK) rc = check_caches(caches, num_caches, a->num_blocks);
   if (rc != PA_OK) return rc;
-  if (!live || !workspace || (a->num_blocks > 0 && (!new_refs || !page_map)) || (a->num_rows > 0 && !new_tables))
+  if (!live || !workspace || (a->num_blocks > 0 && (!new_refs || !page_map)) ||
+      (a->num_rows > 0 && a->max_blocks_per_seq > 0 && !new_tables))
     return PA_ERR_NULL_ARG;
   if (workspace_bytes < pa_fp8_pages_workspace_bytes(PA_PAGES_COMPACT, a->num_blocks, 0)) return PA_ERR_SCRATCH;
   char* ws = (char*)workspace;
