@@ -520,14 +520,15 @@ _NATIVE_ENTRIES = (
     "pa_fp8_free_pages", "pa_fp8_compact_pages",
 )
 _NATIVE = None
+_NATIVE_LIB = None  # the library its calls go to
 
 
 def native():
     """The native call path (``_native``, built with the library), bound to
     the loaded library; None where it is not built or the library is not
     there (the Python launchers then do the whole call, or say so)."""
-    global _NATIVE
-    if _NATIVE is None:
+    global _NATIVE, _NATIVE_LIB
+    if _NATIVE is None or (_NATIVE and _NATIVE_LIB is not _LIB):
         try:
             from . import _native
         except ImportError:
@@ -538,7 +539,7 @@ def native():
         except LibraryNotBuilt:
             return None
         _native.init(tuple(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _NATIVE_ENTRIES), check)
-        _NATIVE = _native
+        _NATIVE, _NATIVE_LIB = _native, lib
     return _NATIVE or None
 
 

@@ -298,9 +298,8 @@ def test_native_path_gives_the_same_bits(monkeypatch):
     both(monkeypatch, run_all)
 
 
-def test_checked_build(checked, monkeypatch):
+def test_checked_build(checked):
     """Table entries outside the cache are passed over and noted."""
-    monkeypatch.setattr(_lib, "_NATIVE", False)  # (bound to the release library)
     t, n, refs = make_pool(8, 6, 64, 16, seed=9, empty=3)
     s = State(t, n, refs, 16)
     s.fork([0, 1], [5, 6])
@@ -320,3 +319,19 @@ def test_checked_build(checked, monkeypatch):
     s.free([0, 1, 2])
     assert _lib.debug_violations(checked) == _lib.VIOLATION_PAGE
     assert not s.refs.any()
+
+
+@pytest.mark.parametrize("rows,width,pages", [(0, 3, 5), (3, 0, 5), (3, 2, 0)])
+def test_empty_states(rows, width, pages):
+    """No rows, no columns, no pages: every entry is left out, but for rows that
+    stay empty."""
+    z = lambda *s: torch.zeros(s, dtype=torch.int32, device=DEV)
+    t, n, r, cache = z(rows, width), z(rows), z(pages), z(pages, 4)
+    assert copy_cache_pages([cache], dev([0, 1]), dev([1, 7])).tolist() == [int(pages > 1), 0]
+    ok = int(rows > 0)
+    assert fork_cache_pages(t, n, r, dev([0]), dev([1]), 16).tolist() == [ok]
+    assert extend_cache_pages([cache], t, n, r, dev([0]), dev([5]), 16).tolist() == [int(rows * width * pages > 0)]
+    assert extend_cache_pages([cache], t, n, r, dev([1]), dev([0]), 16).tolist() == [ok]
+    assert free_cache_pages(t, n, r, dev([0, 9]), 16).tolist() == [ok, 0]
+    out = compact_cache_pages([cache], t, n, r, 16)
+    assert out[0].shape == t.shape and out[1].shape == r.shape and int(out[3]) == 0

@@ -364,10 +364,9 @@ def test_native_path_gives_the_same_bits(monkeypatch, kw):
 
 @pytest.mark.parametrize("kw", [dict(heads=8, kv_heads=2), dict(heads=32, kv_heads=2),
                                 dict(heads=8, kv_heads=2, per_token=True)])
-def test_checked_build(checked, monkeypatch, kw):
+def test_checked_build(checked, kw):
     """Clean calls note nothing; table entries outside the cache are read as the
     nearest page and noted."""
-    monkeypatch.setattr(_lib, "_NATIVE", False)  # (bound to the release library)
     case = make_prefix_case(groups=[ragged(200, 6, 40, 1)], loose=[90], seed=26, poison=False, **kw)
     run(case)
     assert _lib.debug_violations(checked) == 0
