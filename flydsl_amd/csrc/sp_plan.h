@@ -24,7 +24,10 @@
 #define SP_TILE 64          // tokens of a tile
 #define SP_WAVES 4          // waves of a workgroup
 #define SP_MAX_TOKENS (1 << 30)  // of a table row: larger ones count as this
-#define SP_MIN_SHARE 160         // at least a shared tile, and four of a wave's pieces
+// Shortest share of a workgroup: no worker's part may be shorter than a tile (a shared
+// one, or in a wave's quarter a direct one).  4 sequences of a 500-token prefix: 17.6 us
+// (at 160: 18.3, at 224: 18.9).
+#define SP_MIN_SHARE 96
 
 // Sequences and groups of a launch, whose plan (16 bytes a sequence, 20 a group)
 // is held in LDS beside two buffers of a tile: 73 KB of the 160 at head size 128,

@@ -377,3 +377,20 @@ def test_checked_build(checked, kw):
     call(d, out)
     check(dict(d, block_tables=d["block_tables"].clamp(0, nb - 1)), out)
     assert _lib.debug_violations(checked) == _lib.VIOLATION_PAGE
+
+
+def test_scales_and_caches_in_other_forms():
+    """Scales left out or given as numbers, caches as bytes: the same bits as
+    tensors of one value and fp8 caches."""
+    d = to_dev(make_prefix_case(groups=[ragged(100, 3, 30, 1)], seed=27))
+    one = torch.ones(1, device=DEV)
+    want, got = (torch.empty_like(d["query"]) for _ in range(2))
+    call(dict(d, key_scale=one, value_scale=one), want)
+    call(dict(d, key_scale=None, value_scale=None), got)
+    assert torch.equal(got, want)
+    call(dict(d, key_scale=1.0, value_scale=one, key_cache=d["key_cache"].view(torch.uint8),
+              value_cache=d["value_cache"].view(torch.uint8), softmax_scale=d["softmax_scale"]), got)
+    assert torch.equal(got, want)
+    call(dict(d, key_scale=one, value_scale=one, softmax_scale=0), got)  # a whole number
+    call(dict(d, key_scale=one, value_scale=one, softmax_scale=0.0), want)
+    assert torch.equal(got, want)
