@@ -68,7 +68,8 @@ __device__ __forceinline__ bool listed(const int32_t* list, int upto, int v) {
 // Copies
 // ---------------------------------------------------------------------------
 
-constexpr int kUnit = 16384;      // bytes a workgroup copies at a time
+constexpr int kUnit = 4096;       // bytes a wave copies at a time
+constexpr int kWaves = kThreads / 64;
 constexpr int kMaxCaches = 96;    // caches of a launch
 constexpr int kWaveList = 64;     // pairs that every wave checks by itself
 
@@ -140,7 +141,10 @@ __global__ __launch_bounds__(kThreads) void pa_pages_filter_kernel(const int32_t
   status[i] = ok;
 }
 
-// Bytes of `unit` of page s of a cache onto page d.  Written past the caches:
+// Bytes of `unit` of page s of a cache onto page d, by one wave, so that small pages,
+// a token block's scales among them, do not hold a workgroup each (4 KiB pages and
+// 128-byte scales, 16 caches, 2600 moves: 48 us; a workgroup a unit of 16 KiB: 80; large
+// pages alike, a small pool's compaction 15.8 and 14.9 us).  Written past the caches:
 // no one reads them soon; read through them where a page may have several targets
 // (256 copies of 8 pages: 203 us past them, 135 us through).
 __device__ __forceinline__ void copy_unit(const Cache& c, int unit, int s, int d, bool once) {
@@ -148,23 +152,22 @@ __device__ __forceinline__ void copy_unit(const Cache& c, int unit, int s, int d
   const uint32_t n = pa_min(kUnit, (int)(c.bytes - at));
   const uint8_t* from = c.data + (int64_t)s * c.stride + at;
   uint8_t* to = c.data + (int64_t)d * c.stride + at;
-  if (c.unit >= 0) {
-    if (n == kUnit) {  // four loads in flight a thread
-      i32x4 v[4];
-      if (once) {
+  const int lane = threadIdx.x & 63;
+  if (c.unit >= 0) {  // four loads in flight a lane
+    i32x4 v[4];
+    if (n == kUnit && once) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = __builtin_nontemporal_load((const i32x4*)from + k * kThreads + threadIdx.x);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = ((const i32x4*)from)[k * kThreads + threadIdx.x];
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) __builtin_nontemporal_store(v[k], (i32x4*)to + k * kThreads + threadIdx.x);
+      for (int k = 0; k < 4; ++k) v[k] = __builtin_nontemporal_load((const i32x4*)from + k * 64 + lane);
     } else {
-      for (uint32_t k = threadIdx.x; k < n / 16; k += kThreads) ((i32x4*)to)[k] = ((const i32x4*)from)[k];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (16u * (k * 64 + lane) < n) v[k] = ((const i32x4*)from)[k * 64 + lane];
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (16u * (k * 64 + lane) < n) __builtin_nontemporal_store(v[k], (i32x4*)to + k * 64 + lane);
   } else {
-    for (uint32_t k = threadIdx.x; k < n; k += kThreads) to[k] = from[k];
+    for (uint32_t k = lane; k < n; k += 64) to[k] = from[k];
   }
 }
 
@@ -191,7 +194,8 @@ __global__ __launch_bounds__(kThreads) void pa_pages_copy_kernel(const CopyArgs 
     wd = a.dst[lane];
     pa_note(ws >= a.pages || wd >= a.pages, PA_VIOLATION_PAGE);
   }
-  for (int64_t x = blockIdx.x; x < total; x += gridDim.x) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (int64_t x = (int64_t)blockIdx.x * kWaves + wave; x < total; x += (int64_t)gridDim.x * kWaves) {
     const int u = __builtin_amdgcn_readfirstlane((int)(x / n));
     const int i = __builtin_amdgcn_readfirstlane((int)(x - (int64_t)u * n));
     int s, d;
@@ -200,7 +204,7 @@ __global__ __launch_bounds__(kThreads) void pa_pages_copy_kernel(const CopyArgs 
       s = __builtin_amdgcn_readlane(ws, i);
       d = __builtin_amdgcn_readlane(wd, i);
       ok = s >= 0 && s < a.pages && d >= 0 && d < a.pages && !__ballot(lane < n && blocks(s, d, lane, ws, wd, i, a.pages));
-      if (u == 0 && threadIdx.x == 0) a.status[i] = ok;
+      if (u == 0 && lane == 0) a.status[i] = ok;
     } else {
       s = a.src[i];
       d = a.dst[i];
@@ -532,7 +536,8 @@ __global__ __launch_bounds__(kThreads) void pa_pages_extend_kernel(const Extend 
   }
   if (!ok || share < 0) return;
   const int to = free_page(e.pool, sums, start);
-  for (int u = blockIdx.y; u < a.units; u += gridDim.y) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (int u = (int)blockIdx.y * kWaves + wave; u < a.units; u += (int)gridDim.y * kWaves) {
     const int k = cache_of(a, u);
     copy_unit(a.c[k], u - (a.c[k].unit & 0x7fffffff), share, to, false);
   }
@@ -694,7 +699,8 @@ hipError_t launch_copy(const pa_fp8_page_cache* caches, int num, const int32_t* 
     next_caches(caches, num, &at, &a);
     if (a.caches == 0) continue;
     const int64_t total = (int64_t)n * a.units;
-    hipLaunchKernelGGL(pa_pages_copy_kernel, dim3((unsigned)(total < kCopyGrid ? total : kCopyGrid)), dim3(kThreads), 0, s, a);
+    const int64_t groups = (total + kWaves - 1) / kWaves;
+    hipLaunchKernelGGL(pa_pages_copy_kernel, dim3((unsigned)(groups < kCopyGrid ? groups : kCopyGrid)), dim3(kThreads), 0, s, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -808,7 +814,7 @@ extern "C" int pa_fp8_extend_pages(const pa_fp8_page_table_args* a, const pa_fp8
   do {
     CopyArgs c = {};
     next_caches(caches, num_caches, &at, &c);
-    const int y = pa_max(1, pa_min(c.units, kCopyGrid / n));
+    const int y = pa_max(1, pa_min((c.units + kWaves - 1) / kWaves, kCopyGrid / n));
     hipLaunchKernelGGL(pa_pages_extend_kernel, dim3((unsigned)n, (unsigned)y), dim3(kThreads), 0, s, e, c, first);
     err = hipGetLastError();
     if (err != hipSuccess) return (int)err;
